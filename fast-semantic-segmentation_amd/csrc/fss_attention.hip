@@ -1,0 +1,443 @@
+// Attention of queries to the keys and values of another set of tokens (gfx950), one pass over the keys
+// with a running maximum and sum per query:
+//
+//   y[i] = sum_j p[i][j] v[j] / sum_j p[i][j],   p[i][j] = exp(scale * q[i] . k[j] - max_j)
+//
+// The query heads that share a key / value head are rows of one problem (row r = token r / G, head r % G
+// of the group), so keys and values are read once for all of them.  Both products keep a query in
+// ONE matrix column: S^T = K Q^T and O^T = V^T P^T.  A lane of v_mfma_f32_32x32x16 then holds 16 scores
+// of its query (column lane % 32, keys 8 (i / 4) + 4 (lane / 32) + i % 4), the softmax needs one
+// exchange between lanes l and l + 32 and otherwise stays inside a lane, the rescaling of the sums is
+// one factor per lane, and the rounded p are the second product's operand where they are: its 16 keys may
+// be taken in any order as long as V is read in the same one, which the transposing LDS read
+// (ds_read_b64_tr_b16: 4 keys x 16 channels -> 4 keys per lane) does at no cost.
+#include "fss_conv_args.h"
+
+namespace fss {
+namespace {
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef short i16x4_t __attribute__((ext_vector_type(4)));
+
+constexpr int kKeys = 64;              // keys per tile
+
+struct AttnArgs {
+  const char* q;
+  const char* k;
+  const char* v;
+  char* y;
+  const int32_t* lens;
+  const uint8_t* mask;
+  float* part_o;                       // [splits][all rows][head_dim] sums, not yet divided
+  float* part_ml;                      // [splits][all rows][2]: maximum (log2 units), sum
+  long long qs[3], ks[3], vs[3], ys[3], ms[3];
+  int batch, kv_len, kv_heads, group, rows, d, qtiles, splits, negate;
+  float c;                             // |scale| * log2(e)
+};
+
+template <typename T> __device__ __forceinline__ f32x16_t mfma32(const uint4& a, const uint4& b, f32x16_t c) {
+  if constexpr (__is_same(T, f16_t))
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(fss_f16x8, a), __builtin_bit_cast(fss_f16x8, b), c,
+                                                  0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(fss_bf16x8, a),
+                                                   __builtin_bit_cast(fss_bf16x8, b), c, 0, 0, 0);
+}
+
+// Byte layout of a K or V tile in LDS: rows of DP channels, 16-byte chunks exchanged by an XOR with
+// the row so that the lanes of one read spread over all banks.  K is read as one chunk of 8 and
+// more consecutive rows, V as 64 consecutive bytes of 4 consecutive rows.
+template <int DP> struct Tile {
+  static constexpr int kRow = DP * 2, kChunks = DP / 8, kPerLine = kRow < 256 ? 256 / kRow : 1;
+  static constexpr int kBytes = kKeys * kRow;
+  static constexpr int kPieces = kBytes / 1024;
+  static __device__ __forceinline__ int kswz(int row) { return (row / kPerLine) & (kChunks < 16 ? kChunks - 1 : 15); }
+  static __device__ __forceinline__ int vswz(int row) {
+    return ((row / kPerLine) & ((kChunks < 16 ? kChunks : 16) / 4 - 1)) << 2;
+  }
+};
+
+__device__ __forceinline__ float other_half_max(float v) { return fmaxf(v, __shfl_xor(v, 32)); }
+
+template <typename T> __device__ __forceinline__ unsigned pack2_sat(float a, float b) {
+  if constexpr (__is_same(T, f16_t)) {
+    a = a > 65504.f ? 65504.f : a < -65504.f ? -65504.f : a;
+    b = b > 65504.f ? 65504.f : b < -65504.f ? -65504.f : b;
+  }
+  return Half16<T>::pack2(a, b);
+}
+
+template <typename T, int DP, int NW, bool MASK, bool SPLIT>
+__global__ void __launch_bounds__(NW * 64)
+attention_kernel(const AttnArgs a) {
+  typedef Tile<DP> L;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const unsigned smem_base = (unsigned)(size_t)(__attribute__((address_space(3))) char*)smem;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, h = lane >> 5;
+
+  // blocks that share keys and values are neighbours on one XCD (its L2 holds them)
+  const int nwg = gridDim.x, bid = blockIdx.x;
+  const int q8 = nwg >> 3, rr = nwg & 7, xcd = bid & 7;
+  const int wg = (xcd < rr ? xcd * (q8 + 1) : rr * (q8 + 1) + (xcd - rr) * q8) + (bid >> 3);
+  const int qt = wg % a.qtiles, rest = wg / a.qtiles;
+  const int z = rest % a.splits, bh = rest / a.splits;
+  const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
+
+  int len = a.kv_len;
+  if (a.lens != nullptr) len = min(max(a.lens[b], 0), a.kv_len);
+  const int tiles = (len + kKeys - 1) / kKeys;
+  const int per = (tiles + a.splits - 1) / a.splits;
+  const int tile0 = min(z * per, tiles), tile1 = min(tile0 + per, tiles);
+
+  // this lane's query
+  const int r = (qt * NW + wave) * 32 + col;
+  const bool row_ok = r < a.rows;
+  const int token = (row_ok ? r : 0) / a.group, head = hk * a.group + (row_ok ? r : 0) % a.group;
+  uint4 qf[DP / 16];
+  {
+    const char* qp = a.q + 2 * (b * a.qs[0] + token * a.qs[1] + head * a.qs[2]);
+    const unsigned flip = a.negate ? 0x80008000u : 0u;
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) {
+      const int chunk = 2 * s + h;
+      uint4 t = make_uint4(0, 0, 0, 0);
+      if (row_ok && chunk * 8 < a.d) t = *reinterpret_cast<const uint4*>(qp + chunk * 16);
+      qf[s] = make_uint4(t.x ^ flip, t.y ^ flip, t.z ^ flip, t.w ^ flip);
+    }
+  }
+  const uint8_t* mp = nullptr;
+  if constexpr (MASK) mp = a.mask + b * a.ms[0] + token * a.ms[1] + head * a.ms[2];
+  const char* kbase = a.k + 2 * (b * a.ks[0] + hk * a.ks[2]);
+  const char* vbase = a.v + 2 * (b * a.vs[0] + hk * a.vs[2]);
+
+  f32x16_t o[DP / 32];
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i) o[i] = f32x16_t{};
+  float m = -INFINITY, l = 0.f;
+
+  for (int tile = tile0; tile < tile1; ++tile) {
+    const int key0 = tile * kKeys, left = len - key0;
+    // copy the tile: keys at or behind the length and channels behind head_dim are filled with zeros
+    __syncthreads();
+    {
+      const fss_i32x4 rk = dma_resource(kbase + 2 * (long long)key0 * a.ks[1], ~0ull);
+      const fss_i32x4 rv = dma_resource(vbase + 2 * (long long)key0 * a.vs[1], ~0ull);
+      for (int p = wave; p < L::kPieces; p += NW) {
+        const int at = p * 64 + lane, row = at / L::kChunks, phys = at % L::kChunks;
+        const int ck = phys ^ L::kswz(row), cv = phys ^ L::vswz(row);
+        blds16(row < left && ck * 8 < a.d ? (unsigned)(row * 2 * (int)a.ks[1] + ck * 16) : kDmaOutOfRange, rk,
+               smem_base + p * 1024);
+        blds16(row < left && cv * 8 < a.d ? (unsigned)(row * 2 * (int)a.vs[1] + cv * 16) : kDmaOutOfRange, rv,
+               smem_base + L::kBytes + p * 1024);
+      }
+    }
+    wait_vmcnt<0>();
+    __syncthreads();
+
+    // scores of 64 keys
+    f32x16_t s[2];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      s[kt] = f32x16_t{};
+      const int row = kt * 32 + col;
+      const char* base = smem + row * L::kRow;
+#pragma unroll
+      for (int st = 0; st < DP / 16; ++st)
+        s[kt] = mfma32<T>(*reinterpret_cast<const uint4*>(base + ((2 * st + h) ^ L::kswz(row)) * 16), qf[st], s[kt]);
+    }
+    if (left < kKeys || MASK) {
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = kt * 32 + 8 * (i / 4) + 4 * h + i % 4;
+          bool seen = key < left;
+          if constexpr (MASK) seen = seen && mp[seen ? key0 + key : 0] != 0;
+          s[kt][i] = seen ? s[kt][i] : -INFINITY;
+        }
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kt][i]);
+    top = other_half_max(top) * a.c;
+    const float m_new = fmaxf(m, top), m_use = m_new == -INFINITY ? 0.f : m_new;
+    const float alpha = __builtin_amdgcn_exp2f(m - m_use);
+    m = m_new;
+    l *= alpha;
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) o[i] *= alpha;
+    unsigned pf[2][8];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[kt][2 * i], a.c, -m_use));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[kt][2 * i + 1], a.c, -m_use));
+        l += p0 + p1;
+        pf[kt][i] = Half16<T>::pack2(p0, p1);
+      }
+    // O^T += V^T P^T, 16 keys at a time; lane group of 16: 4 keys x 16 channels, transposed on the way
+    const int g16 = lane >> 4, i16 = lane & 15;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      const uint4 pb = make_uint4(pf[ks / 2][4 * (ks & 1)], pf[ks / 2][4 * (ks & 1) + 1], pf[ks / 2][4 * (ks & 1) + 2],
+                                  pf[ks / 2][4 * (ks & 1) + 3]);
+#pragma unroll
+      for (int dt = 0; dt < DP / 32; ++dt) {
+        uint2 half[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int key = ks * 16 + j * 8 + 4 * (g16 >> 1) + (i16 >> 2);
+          const int byte = dt * 64 + (g16 & 1) * 32 + (i16 & 3) * 8;
+          const unsigned at = smem_base + L::kBytes + key * L::kRow + (((byte >> 4) ^ L::vswz(key)) << 4) + (byte & 8);
+          half[j] = __builtin_bit_cast(
+              uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                         (__attribute__((address_space(3))) i16x4_t*)(__attribute__((address_space(3))) char*)(size_t)at));
+        }
+        o[dt] = mfma32<T>(make_uint4(half[0].x, half[0].y, half[1].x, half[1].y), pb, o[dt]);
+      }
+    }
+  }
+
+  l += __shfl_xor(l, 32);
+  const long long prow = ((long long)z * a.batch * a.kv_heads + bh) * a.rows + r;
+  const float f = SPLIT ? 1.f : l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+  char* yp = a.y + 2 * (b * a.ys[0] + token * a.ys[1] + head * a.ys[2]);
+
+  bool done = false;
+  if constexpr (MASK) {
+    // An infinity or a NaN in the value of a key that this query does not see has met p = 0 and
+    // left a NaN.  Such a query's sums are formed again key by key, leaving those keys out.
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) nan = nan || o[i][e] != o[i][e];
+    unsigned long long todo = __ballot(nan && row_ok);
+    unsigned bad = (unsigned)todo | (unsigned)(todo >> 32);
+    done = (bad >> col) & 1;
+    while (bad != 0) {
+      const int at = __ffs((int)bad) - 1;
+      bad &= bad - 1;
+      const int rq = (qt * NW + wave) * 32 + at, tq = rq / a.group, hq = hk * a.group + rq % a.group;
+      const T* qp = reinterpret_cast<const T*>(a.q) + b * a.qs[0] + tq * a.qs[1] + hq * a.qs[2];
+      const uint8_t* mq = a.mask + b * a.ms[0] + tq * a.ms[1] + hq * a.ms[2];
+      const float mx = __shfl(m, at), sum = __shfl(l, at), fq = __shfl(f, at);
+      const float shift = mx == -INFINITY ? 0.f : mx;
+      constexpr int PER = (DP + 63) / 64;
+      float acc[PER];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+      for (int j = tile0 * kKeys; j < min(tile1 * kKeys, len); ++j) {
+        if (mq[j] == 0) continue;
+        const T* kp = reinterpret_cast<const T*>(kbase) + j * a.ks[1];
+        const T* vp = reinterpret_cast<const T*>(vbase) + j * a.vs[1];
+        float dot = 0.f;
+        for (int i = lane; i < a.d; i += 64) dot = fmaf(ElemTraits<T>::load(qp + i), ElemTraits<T>::load(kp + i), dot);
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) dot += __shfl_xor(dot, x);
+        const float p = Half16<T>::value(
+            Half16<T>::bits(__builtin_amdgcn_exp2f(fmaf(a.negate ? -dot : dot, a.c, -shift))));
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+          if (lane + 64 * i < a.d) acc[i] = fmaf(p, ElemTraits<T>::load(vp + lane + 64 * i), acc[i]);
+      }
+      const long long pq = ((long long)z * a.batch * a.kv_heads + bh) * a.rows + rq;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int ch = lane + 64 * i;
+        if (ch < a.d) {
+          if constexpr (SPLIT) a.part_o[pq * a.d + ch] = acc[i];
+          else
+            reinterpret_cast<unsigned short*>(a.y)[b * a.ys[0] + tq * a.ys[1] + hq * a.ys[2] + ch] =
+                (unsigned short)pack2_sat<T>(acc[i] * fq, 0.f);
+        }
+      }
+      (void)sum;
+    }
+  }
+  if (!row_ok) return;
+  if constexpr (SPLIT) {
+    if (h == 0) {
+      a.part_ml[prow * 2] = m;
+      a.part_ml[prow * 2 + 1] = l;
+    }
+  }
+  if (done) return;
+#pragma unroll
+  for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int ch = dt * 32 + 8 * j + 4 * h;
+      if (ch >= a.d) continue;
+      const float v0 = o[dt][4 * j], v1 = o[dt][4 * j + 1], v2 = o[dt][4 * j + 2], v3 = o[dt][4 * j + 3];
+      if constexpr (SPLIT)
+        *reinterpret_cast<float4*>(a.part_o + prow * a.d + ch) = make_float4(v0, v1, v2, v3);
+      else
+        *reinterpret_cast<uint2*>(yp + ch * 2) =
+            l == 0.f ? make_uint2(0, 0) : make_uint2(pack2_sat<T>(v0 * f, v1 * f), pack2_sat<T>(v2 * f, v3 * f));
+    }
+}
+
+// Joins the pieces of the key axis: weights 2^(m_z - max m), in index order.  One thread per 4 channels.
+template <typename T>
+__global__ void __launch_bounds__(256) attention_join_kernel(const AttnArgs a, long long all_rows) {
+  const int quads = a.d / 4;
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const long long row = i / quads;
+  if (row >= all_rows) return;
+  const int ch = (int)(i % quads) * 4;
+  float top = -INFINITY;
+  for (int z = 0; z < a.splits; ++z) top = fmaxf(top, a.part_ml[(z * all_rows + row) * 2]);
+  if (top == -INFINITY) top = 0.f;
+  float l = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int z = 0; z < a.splits; ++z) {
+    const float* ml = a.part_ml + (z * all_rows + row) * 2;
+    const float w = __builtin_amdgcn_exp2f(ml[0] - top);
+    const float4 t = *reinterpret_cast<const float4*>(a.part_o + (z * all_rows + row) * a.d + ch);
+    if (ml[1] == 0.f) continue;          // this piece holds no key of the query
+    l = fmaf(w, ml[1], l);
+    v[0] = fmaf(w, t.x, v[0]); v[1] = fmaf(w, t.y, v[1]); v[2] = fmaf(w, t.z, v[2]); v[3] = fmaf(w, t.w, v[3]);
+  }
+  const long long bh = row / a.rows;
+  const int r = (int)(row % a.rows);
+  const int b = (int)(bh / a.kv_heads), head = (int)(bh % a.kv_heads) * a.group + r % a.group;
+  const float f = l == 0.f ? 0.f : 1.f / l;
+  *reinterpret_cast<uint2*>(a.y + 2 * (b * a.ys[0] + r / a.group * a.ys[1] + head * a.ys[2] + ch)) =
+      make_uint2(pack2_sat<T>(v[0] * f, v[1] * f), pack2_sat<T>(v[2] * f, v[3] * f));
+}
+
+struct Shape {
+  int waves, qtiles, splits;
+};
+
+// Queries of a workgroup: 32 per wave.  Where the query tiles do not fill the chip (256 compute units,
+// two workgroups of four waves or eight of one wave each) the key axis is cut into pieces of at least
+// 256 keys, joined by a second launch.
+Shape shape_of(const fss_attention_desc& d) {
+  Shape s;
+  const long long rows = (long long)d.q_len * (d.q_heads / d.kv_heads);
+  s.waves = rows > 32 ? 4 : 1;
+  s.qtiles = ceil_div(rows, 32 * s.waves);
+  const long long blocks = (long long)d.batch * d.kv_heads * s.qtiles;
+  const long long want = s.waves == 4 ? 512 : 2048;
+  long long splits = want / blocks, most = ceil_div(d.kv_len, 256);
+  if (splits > most) splits = most;
+  s.splits = splits > 1 ? (int)splits : 1;
+  return s;
+}
+
+int check_desc(const fss_attention_desc* d) {
+  FSS_REQUIRE(d != nullptr, "null descriptor");
+  FSS_REQUIRE(d->dtype == FSS_BF16 || d->dtype == FSS_F16, "dtype must be FSS_BF16 or FSS_F16");
+  FSS_REQUIRE(d->batch >= 0 && d->q_len >= 0 && d->kv_len >= 0, "negative size");
+  FSS_REQUIRE(d->kv_heads > 0 && d->q_heads > 0 && d->q_heads % d->kv_heads == 0,
+              "q_heads must be a positive multiple of kv_heads");
+  FSS_REQUIRE(d->head_dim > 0 && d->head_dim <= 256 && d->head_dim % 8 == 0,
+              "head_dim must be a multiple of 8 and at most 256");
+  FSS_REQUIRE(d->scale - d->scale == 0.f, "scale must be finite");
+  FSS_REQUIRE((long long)d->q_len * (d->q_heads / d->kv_heads) < 0x7fff0000LL && d->kv_len < 0x7fff0000, "too long");
+  FSS_REQUIRE((long long)d->batch * d->kv_heads *
+                      ((long long)d->q_len * (d->q_heads / d->kv_heads) / 32 + 1) < 0x7fff0000LL,
+              "too many query tiles");
+  return 0;
+}
+
+size_t workspace_of(const fss_attention_desc& d, const Shape& s) {
+  return s.splits == 1 ? 0 : (size_t)s.splits * d.batch * d.q_len * d.q_heads * (d.head_dim + 2) * 4;
+}
+
+template <typename T, int DP, int NW>
+int launch(const AttnArgs& a, const Shape& s, hipStream_t stream) {
+  const dim3 grid((unsigned)((long long)a.batch * a.kv_heads * a.qtiles * a.splits));
+  const size_t lds = 2 * Tile<DP>::kBytes;
+#define FSS_ATTN(MASK, SPLIT)                                                                                       \
+  do {                                                                                                              \
+    FSS_CHECK_HIP(hipFuncSetAttribute((const void*)attention_kernel<T, DP, NW, MASK, SPLIT>,                        \
+                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));                       \
+    hipLaunchKernelGGL((attention_kernel<T, DP, NW, MASK, SPLIT>), grid, dim3(NW * 64), lds, stream, a);            \
+  } while (0)
+  if (a.mask != nullptr) {
+    if (s.splits > 1) FSS_ATTN(true, true); else FSS_ATTN(true, false);
+  } else {
+    if (s.splits > 1) FSS_ATTN(false, true); else FSS_ATTN(false, false);
+  }
+#undef FSS_ATTN
+  FSS_LAUNCH_CHECK();
+  return 0;
+}
+
+template <typename T>
+int launch_type(const AttnArgs& a, const Shape& s, hipStream_t stream) {
+#define FSS_DP(DP) return s.waves == 4 ? launch<T, DP, 4>(a, s, stream) : launch<T, DP, 1>(a, s, stream)
+  if (a.d <= 32) FSS_DP(32);
+  if (a.d <= 64) FSS_DP(64);
+  if (a.d <= 128) FSS_DP(128);
+  FSS_DP(256);
+#undef FSS_DP
+}
+
+}  // namespace
+}  // namespace fss
+
+using namespace fss;
+
+extern "C" {
+
+int fss_cross_attention_workspace_bytes(const fss_attention_desc* desc, size_t* bytes) {
+  FSS_REQUIRE(bytes != nullptr, "null argument");
+  if (int e = check_desc(desc)) return e;
+  *bytes = desc->batch == 0 || desc->q_len == 0 ? 0 : workspace_of(*desc, shape_of(*desc));
+  return 0;
+}
+
+int fss_cross_attention(const fss_attention_desc* desc, const void* q, const void* k, const void* v,
+                        const int32_t* kv_lens, const uint8_t* mask, void* y, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+  if (int e = check_desc(desc)) return e;
+  const fss_attention_desc& d = *desc;
+  if (d.batch == 0 || d.q_len == 0) return 0;
+  FSS_REQUIRE(q && y && ((k && v) || d.kv_len == 0), "null argument");
+  for (int i = 0; i < 3; ++i) {
+    const int64_t st[4] = {d.q_stride[i], d.k_stride[i], d.v_stride[i], d.y_stride[i]};
+    for (int t = 0; t < 4; ++t)
+      FSS_REQUIRE(st[t] >= 0 && st[t] % 8 == 0 && (i != 1 || st[t] < (1 << 24)),
+                  "strides must be multiples of 8 and not negative, token strides below 2^24");
+    FSS_REQUIRE(mask == nullptr || d.mask_stride[i] >= 0, "negative mask stride");
+  }
+  FSS_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)y | (uintptr_t)workspace) & 15) == 0 &&
+                  ((uintptr_t)kv_lens & 3) == 0, "unaligned pointer");
+  const Shape s = shape_of(d);
+  const size_t need = workspace_of(d, s);
+  FSS_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), "workspace too small");
+  AttnArgs a;
+  a.q = (const char*)q; a.k = (const char*)k; a.v = (const char*)v; a.y = (char*)y;
+  a.lens = kv_lens; a.mask = mask;
+  for (int i = 0; i < 3; ++i) {
+    a.qs[i] = d.q_stride[i]; a.ks[i] = d.k_stride[i]; a.vs[i] = d.v_stride[i]; a.ys[i] = d.y_stride[i];
+    a.ms[i] = d.mask_stride[i];
+  }
+  a.batch = d.batch; a.kv_len = d.kv_len; a.kv_heads = d.kv_heads; a.group = d.q_heads / d.kv_heads;
+  a.rows = d.q_len * a.group; a.d = d.head_dim; a.qtiles = s.qtiles; a.splits = s.splits;
+  a.negate = d.scale < 0.f;
+  // (a scale of 0 gives equal scores; the smallest float in its place keeps 0 * infinity out)
+  a.c = fmaxf(fabsf(d.scale) * 1.44269504088896340736f, 1.17549435e-38f);
+  const long long all_rows = (long long)d.batch * d.q_len * d.q_heads;
+  a.part_o = (float*)workspace;
+  a.part_ml = a.part_o + (need == 0 ? 0 : s.splits * all_rows * d.head_dim);
+  hipStream_t st = (hipStream_t)stream;
+  const int e = d.dtype == FSS_F16 ? launch_type<f16_t>(a, s, st) : launch_type<bf16_t>(a, s, st);
+  if (e != 0 || s.splits == 1) return e;
+  const long long threads = all_rows * (d.head_dim / 4);
+  FSS_REQUIRE((threads + 255) / 256 < 0x7fffffffLL, "too many rows");
+  const dim3 grid((unsigned)((threads + 255) / 256));
+  if (d.dtype == FSS_F16) hipLaunchKernelGGL(attention_join_kernel<f16_t>, grid, dim3(256), 0, st, a, all_rows);
+  else hipLaunchKernelGGL(attention_join_kernel<bf16_t>, grid, dim3(256), 0, st, a, all_rows);
+  FSS_LAUNCH_CHECK();
+  return 0;
+}
+
+}  // extern "C"

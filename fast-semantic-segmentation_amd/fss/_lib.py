@@ -31,6 +31,19 @@ class ConvDesc(ctypes.Structure):
         'y_ld', 'res_ld', 'k_pad', 'cout_pad', 'config')]
 
 
+class MatmulFp8Desc(ctypes.Structure):
+    """Mirror of `fss_matmul_fp8_desc`."""
+    _fields_ = ([(n, ctypes.c_int64) for n in ('rows', 'x_ld', 'x_scale_ld', 'w_ld', 'w_scale_ld', 'res_ld', 'y_ld')] +
+                [(n, ctypes.c_int32) for n in ('cout', 'k', 'act', 'out_dtype')])
+
+
+class AttentionDesc(ctypes.Structure):
+    """Mirror of `fss_attention_desc`."""
+    _fields_ = ([(n, ctypes.c_int32) for n in ('batch', 'q_len', 'kv_len', 'q_heads', 'kv_heads', 'head_dim', 'dtype')] +
+                [('scale', ctypes.c_float)] +
+                [(n, ctypes.c_int64 * 3) for n in ('q_stride', 'k_stride', 'v_stride', 'y_stride', 'mask_stride')])
+
+
 # name -> (restype, argtypes); must list every symbol of include/fss.h
 PROTOTYPES = {
     'fss_last_error': (ctypes.c_char_p, []),
@@ -98,6 +111,12 @@ PROTOTYPES = {
                                   c_float_p, c_float_p, c_int, c_void_p]),
     'fss_upsample_argmax': (c_int, [c_void_p, c_void_p, c_void_p] + [c_int] * 7 + [c_void_p]),
     'fss_label_lut': (c_int, [c_void_p, c_void_p, c_void_p] + [c_int] * 7 + [c_void_p]),
+    'fss_quantize_fp8': (c_int, [c_void_p, ctypes.c_longlong, c_void_p, ctypes.c_longlong, c_void_p, ctypes.c_longlong,
+                                 ctypes.c_longlong, c_int, c_int, c_int, c_void_p]),
+    'fss_matmul_fp8_workspace_bytes': (c_int, [ctypes.POINTER(MatmulFp8Desc), ctypes.POINTER(c_size_t)]),
+    'fss_matmul_fp8': (c_int, [ctypes.POINTER(MatmulFp8Desc)] + [c_void_p] * 8 + [c_size_t, c_void_p]),
+    'fss_cross_attention_workspace_bytes': (c_int, [ctypes.POINTER(AttentionDesc), ctypes.POINTER(c_size_t)]),
+    'fss_cross_attention': (c_int, [ctypes.POINTER(AttentionDesc)] + [c_void_p] * 7 + [c_size_t, c_void_p]),
     'fss_confusion_accumulate': (c_int, [c_void_p, c_void_p, c_size_t, c_int, c_int, c_void_p, c_void_p]),
 }
 

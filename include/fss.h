@@ -456,6 +456,87 @@ int fss_confusion_accumulate(const uint8_t* pred, const uint8_t* labels,
                              size_t count, int num_classes, int ignore_label,
                              int64_t* cm, void* stream);
 
+/* ------------------------------------------- 8-bit products and cross attention
+ *
+ * What a decoder on top of the feature maps needs next to the convolutions: projections in 8-bit
+ * floating point and attention of queries (pixels, object queries, single tokens) to the tokens of
+ * another map.  The reference has no counterpart.  The conventions above hold; the current
+ * device is the one that owns the stream and the tensors, outputs overlap no input, and a
+ * workspace belongs to one call until that call's work is done (two captured graphs that may
+ * run at once need one each).  Zero rows, queries or batch entries: success, nothing launched. */
+
+/* q = x in 8-bit floating point (OCP e4m3: 4 exponent bits, 3 mantissa bits, largest 448) with a
+ * float scale per block of `block_rows` (1 or 128) rows x 128 columns, x ~ q * scale:
+ *   a = max(largest |x| of the block, 2^-100),  scale = a / 448,
+ *   q = (x * (448 / a)) rounded to nearest even, in float.
+ * x: [rows][cols] of `dtype` (FSS_F32 | FSS_BF16 | FSS_F16 | FSS_F32_BF16X3), cols a multiple of 16,
+ * row stride x_ld a multiple of 16 bytes (FSS_F32_BF16X3: of 32); q: row stride q_ld a multiple of 16;
+ * scales: [ceil(cols/128)][ceil(rows/block_rows)], stride scale_ld between column blocks (rows
+ * next to each other: what the product reads as one line).  The last blocks may be smaller.  A block
+ * that holds an infinity or a NaN becomes NaN as a whole, values and scale.
+ * block_rows 1 is for activations, 128 for weights [cout][k]. */
+int fss_quantize_fp8(const void* x, long long x_ld, void* q, long long q_ld, float* scales,
+                     long long scale_ld, long long rows, int cols, int block_rows, int dtype,
+                     void* stream);
+
+typedef struct fss_matmul_fp8_desc {
+  int64_t rows;              /* rows of x and y: pixels, queries, one token  */
+  int64_t x_ld, x_scale_ld;  /* strides of x and its scales, see above       */
+  int64_t w_ld, w_scale_ld;
+  int64_t res_ld, y_ld;      /* row strides in elements (>= cout)            */
+  int32_t cout, k;           /* w: [cout][k]; k a multiple of 16             */
+  int32_t act;               /* FSS_ACT_*                                    */
+  int32_t out_dtype;         /* FSS_F32 | FSS_BF16 | FSS_F16 | FSS_F32_BF16X3
+                                (y and residual; the last: cout, y_ld and
+                                res_ld multiples of 8)                        */
+} fss_matmul_fp8_desc;
+
+/* Device bytes fss_matmul_fp8 needs as its workspace for these sizes (often 0): float partial
+ * sums where few rows meet a long k and the k axis is split. */
+int fss_matmul_fp8_workspace_bytes(const fss_matmul_fp8_desc* desc, size_t* bytes);
+
+/* y = act( sum_b x_scale[b][m] * w_scale[b][n / 128] * (x[m][b] . w[n][b]) + bias[n] [+ residual[m][n]] )
+ * over the blocks b of 128 along k: the product of two tensors fss_quantize_fp8 made, x with
+ * block_rows 1 and w with block_rows 128, with fss_conv2d_nhwc's epilogue.  The products of a block are
+ * summed on the matrix cores, blocks are scaled and summed in float, the result is rounded once, to
+ * out_dtype (FSS_F16 saturates).  With 16-bit outputs the 8-bit matrix instructions are used, which drop
+ * what lies below 2^-13 of the largest of 8 products (2e-5 of the result's size); with FSS_F32 and
+ * FSS_F32_BF16X3 the same values go through the half-precision ones, which sum to float accuracy.  x, w, bias and workspace: 16-byte aligned, y and
+ * residual aligned to their element (FSS_F32_BF16X3: 32 bytes).  bias, residual: NULL = none. */
+int fss_matmul_fp8(const fss_matmul_fp8_desc* desc, const void* x, const float* x_scales,
+                   const void* w, const float* w_scales, const float* bias, const void* residual,
+                   void* y, void* workspace, size_t workspace_bytes, void* stream);
+
+typedef struct fss_attention_desc {
+  int32_t batch, q_len, kv_len;
+  int32_t q_heads, kv_heads;  /* q_heads a multiple of kv_heads: query head h
+                                 reads key / value head h / (q_heads / kv_heads) */
+  int32_t head_dim;           /* a multiple of 8, at most 256                  */
+  int32_t dtype;              /* FSS_BF16 | FSS_F16 (q, k, v and y)             */
+  float scale;                /* of the scores, usually head_dim^-1/2           */
+  int64_t q_stride[3];        /* batch, token, head, in elements: multiples    */
+  int64_t k_stride[3];        /* of 8, not negative, token strides below 2^24  */
+  int64_t v_stride[3];
+  int64_t y_stride[3];
+  int64_t mask_stride[3];     /* batch, query, head, in bytes; 0 = shared       */
+} fss_attention_desc;
+
+/* Device bytes fss_cross_attention needs as its workspace for these sizes (0 where the queries
+ * alone fill the chip): partial results of the pieces of the key axis. */
+int fss_cross_attention_workspace_bytes(const fss_attention_desc* desc, size_t* bytes);
+
+/* y[b,i,h] = sum_j p[j] v[b,j,h'] / sum_j p[j],  p[j] = exp(scale * q[b,i,h] . k[b,j,h'] - max)
+ * over the keys j < kv_lens[b] (NULL: kv_len; values are clamped to 0 .. kv_len) whose
+ * mask[b,i,h,j] is not 0 (uint8, consecutive along j; NULL: all).  A query without any such key
+ * gets zeros.  Keys and values at or behind kv_lens[b] are not read; a masked key has no effect
+ * whatever its key and value hold, infinities and NaN included.  Scores, maximum, sums and
+ * the output are accumulated in float; p is rounded to `dtype` for the product with v, y once at the
+ * end (FSS_F16 saturates).  q, k, v, y, workspace: 16-byte aligned.  kv_lens is read on the device, so a captured
+ * call follows its later contents. */
+int fss_cross_attention(const fss_attention_desc* desc, const void* q, const void* k, const void* v,
+                        const int32_t* kv_lens, const uint8_t* mask, void* y, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
