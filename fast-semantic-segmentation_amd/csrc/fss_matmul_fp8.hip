@@ -12,7 +12,7 @@
 // same one), so a lane simply takes 16-byte pieces g and g + 4 of its row's 128 bytes.
 #include <type_traits>
 
-#include "fss_common.h"
+#include "fss_conv_args.h"
 
 namespace fss {
 namespace {
@@ -78,15 +78,17 @@ __device__ __forceinline__ fss_f32x4 mma(const Block<T>& a, const Block<T>& b) {
   }
 }
 
-// (comparisons instead of min / max: a NaN stays one)
-__device__ __forceinline__ float activate(float v, int act) {
-  if (act != FSS_ACT_NONE) v = v < 0.f ? 0.f : v;
-  if (act == FSS_ACT_RELU6) v = v > 6.f ? 6.f : v;
-  return v;
+// Bounds of the activation, for half precision cut to its largest value; minimum and maximum that keep a
+// NaN (v_minimum3_f32, v_maximum3_f32).
+struct Limits {
+  float lo, hi;
+};
+template <typename T> __device__ __forceinline__ Limits limits_of(int act) {
+  const float top = __is_same(T, f16_t) ? 65504.f : INFINITY;
+  return {act == FSS_ACT_NONE ? -top : 0.f, act == FSS_ACT_RELU6 ? 6.f : top};
 }
-template <typename T> __device__ __forceinline__ float storable(float v) { return v; }
-template <> __device__ __forceinline__ float storable<f16_t>(float v) {
-  return v > 65504.f ? 65504.f : v < -65504.f ? -65504.f : v;
+__device__ __forceinline__ float clip(float v, const Limits& l) {
+  return __builtin_elementwise_minimum(__builtin_elementwise_maximum(v, l.lo), l.hi);
 }
 
 template <typename T> __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
@@ -122,99 +124,352 @@ template <typename T> __device__ __forceinline__ void store1(T* p, float v) {
   else ElemTraits<T>::store(p, v);
 }
 
-// Bias, residual, activation and store of 8 consecutive channels of one row.
-template <typename T>
-__device__ __forceinline__ void finish8(const MmArgs& a, long long row, int c0, float (&v)[8]) {
-  if (row >= a.rows || c0 >= a.cout) return;
+// Bias, residual, activation and store of 8 consecutive channels of one row that exists.  VEC: cout and
+// the strides allow 16-byte accesses.  (Two kernels instead of a branch: a launch that does little
+// is bound by fetching its instructions.)
+template <typename T, bool VEC>
+__device__ __forceinline__ void finish8(const MmArgs& a, const Limits& lim, long long row, int c0, float (&v)[8]) {
   T* y = reinterpret_cast<T*>(a.y) + row * a.y_ld + c0;
-  const T* res = a.res != nullptr ? reinterpret_cast<const T*>(a.res) + row * a.res_ld + c0 : nullptr;
-  if (a.vec && c0 + 8 <= a.cout) {
+  const T* res = reinterpret_cast<const T*>(a.res) + row * a.res_ld + c0;
+  if constexpr (VEC) {
     if (a.bias != nullptr) {
       float b[8];
       load8(a.bias + c0, b);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += b[e];
     }
-    if (res != nullptr) {
+    if (a.res != nullptr) {
       float r[8];
       load8(res, r);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += r[e];
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = storable<T>(activate(v[e], a.act));
+    for (int e = 0; e < 8; ++e) v[e] = clip(v[e], lim);
     store8(y, v);
-    return;
-  }
+  } else {
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (c0 + e < a.cout) {
-      float t = v[e];
-      if (a.bias != nullptr) t += a.bias[c0 + e];
-      if (res != nullptr) t += ElemTraits<T>::load(res + e);
-      store1(y + e, storable<T>(activate(t, a.act)));
-    }
+    for (int e = 0; e < 8; ++e)
+      if (c0 + e < a.cout) {
+        float t = v[e];
+        if (a.bias != nullptr) t += a.bias[c0 + e];
+        if (a.res != nullptr) t += ElemTraits<T>::load(res + e);
+        store1(y + e, clip(t, lim));
+      }
+  }
 }
 
 // ------------------------------------------------------------------------------- few rows
-// 32 channels x 16 rows per workgroup, the blocks of k dealt to its 4 waves, operands straight from
-// memory to registers; the waves' sums are added in LDS in a fixed order.
-constexpr int kFewWaves = 4;
+// 32 channels x 16 rows per workgroup, the blocks of k dealt to its 16 waves, operands straight from
+// memory to registers (lanes without a row, a channel or a piece of k read zeros past the buffer's
+// end); the waves' sums are added in LDS in a fixed order, one output per thread.  Latency-bound: one
+// round trip per 2048 of k, and few instructions, as fetching them is most of a launch this small.
+constexpr int kFewWaves = 16;
+constexpr unsigned kMmBytes = 0xe0000000u;       // window of a tile's rows: 256 rows of at most 2^23 bytes
+constexpr unsigned kMmOutside = 0xf0000000u;     // an offset past it that stays past it for every k
+
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ uint4 load_piece(__amdgpu_buffer_rsrc_t rsrc, unsigned off) {
+  return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)off, 0, 0));
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t window(const void* base, unsigned bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00020000);
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kFewWaves * 64)
 matmul_fp8_few_kernel(const MmArgs a, int chan_tiles) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, g = lane >> 4;
-  const long long wg = blockIdx.x;
-  const int n0 = (int)(wg % chan_tiles) * 32;
-  const long long m0 = wg / chan_tiles * 16;
+  const int wg = blockIdx.x;
+  const int n0 = wg % chan_tiles * 32;
+  const long long m0 = (long long)(wg / chan_tiles) * 16;
+  const int rows_left = (int)min(16ll, a.rows - m0), chans_left = a.cout - n0;
 
-  const long long row = m0 + r;
-  const bool row_ok = row < a.rows;
-  const int ch0 = n0 + 8 * (r >> 2) + (r & 3), ch1 = ch0 + 4;
-  const bool ch0_ok = ch0 < a.cout, ch1_ok = ch1 < a.cout;
-  const char* px = a.x + (row_ok ? row : 0) * a.x_ld + g * 16;
-  const char* pw0 = a.w + (long long)(ch0_ok ? ch0 : 0) * a.w_ld + g * 16;
-  const char* pw1 = a.w + (long long)(ch1_ok ? ch1 : 0) * a.w_ld + g * 16;
-  const float* psx = a.sx + (row_ok ? row : 0);
-  const float* psw = a.sw + (n0 >> 7);
+  const __amdgpu_buffer_rsrc_t bx = window(a.x + m0 * a.x_ld, kMmBytes);
+  const __amdgpu_buffer_rsrc_t bw = window(a.w + (long long)n0 * a.w_ld, kMmBytes);
+  const int ch = 8 * (r >> 2) + (r & 3);
+  const unsigned x0 = r < rows_left ? (unsigned)(r * (int)a.x_ld) : kMmOutside;
+  const unsigned w0 = ch < chans_left ? (unsigned)(ch * (int)a.w_ld) : kMmOutside;
+  const unsigned w1 = ch + 4 < chans_left ? (unsigned)((ch + 4) * (int)a.w_ld) : kMmOutside;
 
-  fss_f32x4 acc0 = {0.f, 0.f, 0.f, 0.f}, acc1 = {0.f, 0.f, 0.f, 0.f};
-  const uint4 zero = make_uint4(0, 0, 0, 0);
-  auto piece = [&](const char* p, int off, bool ok) {
-    return ok && off + g * 16 < a.k ? *reinterpret_cast<const uint4*>(p + off) : zero;
-  };
+  fss_f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
   for (int kb = wave; kb < a.kblocks; kb += kFewWaves) {
-    const int o0 = kb * 128, o1 = o0 + 64;
-    Block<T> fx, f0, f1;
-    fx.set(piece(px, o0, row_ok), piece(px, o1, row_ok));
-    f0.set(piece(pw0, o0, ch0_ok), piece(pw0, o1, ch0_ok));
-    f1.set(piece(pw1, o0, ch1_ok), piece(pw1, o1, ch1_ok));
-    const float s = (row_ok ? psx[kb * a.x_scale_ld] : 0.f) * psw[kb * a.w_scale_ld];
-    const fss_f32x4 p0 = mma<T>(f0, fx), p1 = mma<T>(f1, fx);
+    const int o0 = kb * 128 + g * 16, o1 = o0 + 64;
+    const unsigned t0 = o0 < a.k ? (unsigned)o0 : kMmOutside, t1 = o1 < a.k ? (unsigned)o1 : kMmOutside;
+    auto at = [](unsigned row, unsigned k) { return row >= kMmOutside || k >= kMmOutside ? kMmOutside : row + k; };
+    const float sx = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
+                                                   window(a.sx + kb * a.x_scale_ld + m0, rows_left * 4), r * 4, 0, 0));
+    const float sw = a.sw[kb * a.w_scale_ld + (n0 >> 7)];
+    Block<T> fx, f[2];
+    fx.set(load_piece(bx, at(x0, t0)), load_piece(bx, at(x0, t1)));
+    f[0].set(load_piece(bw, at(w0, t0)), load_piece(bw, at(w0, t1)));
+    f[1].set(load_piece(bw, at(w1, t0)), load_piece(bw, at(w1, t1)));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      acc0[i] = fmaf(p0[i], s, acc0[i]);
-      acc1[i] = fmaf(p1[i], s, acc1[i]);
+    for (int t = 0; t < 2; ++t) {
+      const fss_f32x4 p = mma<T>(f[t], fx);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[t][i] = fmaf(p[i], sx * sw, acc[t][i]);
     }
   }
   __shared__ float part[kFewWaves][8][64];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    part[wave][i][lane] = acc0[i];
-    part[wave][4 + i][lane] = acc1[i];
-  }
+  for (int e = 0; e < 8; ++e) part[wave][e][lane] = acc[e >> 2][e & 3];
   __syncthreads();
-  if (wave != 0) return;
-  float v[8];
+  if (wave >= 8) return;
+  float v = 0.f;
+  for (int i = 0; i < min(kFewWaves, a.kblocks); ++i) v += part[i][wave][lane];
+  const int c = 8 * g + wave;
+  if (r >= rows_left || c >= chans_left) return;
+  if (a.bias != nullptr) v += a.bias[n0 + c];
+  if (a.res != nullptr) v += ElemTraits<T>::load(reinterpret_cast<const T*>(a.res) + (m0 + r) * a.res_ld + n0 + c);
+  store1(reinterpret_cast<T*>(a.y) + (m0 + r) * a.y_ld + n0 + c, clip(v, limits_of<T>(a.act)));
+}
+
+// ------------------------------------------------------------------------------ many rows
+// BM rows x BN channels per workgroup of WM x WN waves.  Blocks of k (128 bytes of every row) are copied to
+// a ring of NS LDS stages, NS - 1 blocks ahead of the products; 16-byte chunks of a row are exchanged by
+// an XOR with the row, so that a fragment's reads spread over all banks.  Rows and channels past the
+// end and the tail of k are filled with zeros by out-of-range offsets.  The
+// scales travel in the same stages (a scalar load in the loop would make every LDS read wait for memory,
+// as both count on one counter): 64 rows per wave, and the tile's weight scales in the next one.
+template <int BM, int BN, int WM, int WN, int WK, int NS> struct MmTile {
+  static constexpr int kThreads = 64 * WM * WN * WK, kWaves = WM * WN;
+  static constexpr int TJ = BM / WM / 16, TI = BN / WN / 16;
+  static constexpr int kXPieces = BM / 8 / kWaves, kWPieces = BN / 8 / kWaves;   // 1 KiB each, per wave
+  static constexpr int kPieces = kXPieces + kWPieces;
+  static constexpr int kSPieces = BM / 64 + 1;                                   // 256 bytes each, one per wave
+  static constexpr int kXBytes = BM * 128, kWBytes = BN * 128;
+  static constexpr int kStage = kXBytes + kWBytes + kSPieces * 256;
+  static constexpr int kLds = NS * WK * kStage;
+  static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0 && TI % 2 == 0 && kSPieces <= kWaves &&
+                    BM % 64 == 0 && BN % (TI * 16) == 0 && 128 % (TI * 16) == 0, "tile shape");
+  static_assert(kLds <= 160 * 1024 && (NS - 2) * (kPieces + 1) <= 63 && NS >= 2 && NS <= 4, "ring");
+};
+
+// 64 lanes x 4 bytes to the 256 bytes of LDS at lds_dst
+__device__ __forceinline__ void blds4(unsigned voff, fss_i32x4 rsrc, unsigned lds_dst) {
+  asm volatile(
+      "s_mov_b32 m0, %2\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dword %0, %1, 0 offen lds"
+      :
+      : "v"(voff), "s"(rsrc), "s"(lds_dst)
+      : "memory", "m0");
+}
+
+template <typename T, bool VEC, int BM, int BN, int WM, int WN, int WK, int NS>
+__global__ void __launch_bounds__(64 * WM * WN * WK, 2)
+matmul_fp8_tile_kernel(const MmArgs a, int tiles_n) {
+  typedef MmTile<BM, BN, WM, WN, WK, NS> L;
+  constexpr int TJ = L::TJ, TI = L::TI;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const int lane = threadIdx.x & 63, waves = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wk = waves / L::kWaves, wave = waves % L::kWaves;      // group along k, wave of the group
+  const int wm = wave / WN, wn = wave % WN;
+  char* ring = smem + wk * NS * L::kStage;                         // each group has a ring of its own
+  const unsigned ring_base = (unsigned)(size_t)(__attribute__((address_space(3))) char*)ring;
+
+  // the tiles of one XCD are neighbours, taken in columns of 8: what runs at a time shares rows
+  // and channels in its L2
+  const int nwg = gridDim.x, bid = blockIdx.x;
+  const int q8 = nwg >> 3, rr = nwg & 7, xcd = bid & 7;
+  const int wg = (xcd < rr ? xcd * (q8 + 1) : rr * (q8 + 1) + (xcd - rr) * q8) + (bid >> 3);
+  const int tiles_m = nwg / tiles_n, band = wg / (8 * tiles_n), in_band = wg - band * 8 * tiles_n;
+  const int band_m = min(8, tiles_m - band * 8);
+  const long long m0 = (long long)(band * 8 + in_band % band_m) * BM;
+  const int n0 = in_band / band_m * BN;
+  const int rows_left = (int)min((long long)BM, a.rows - m0), chans_left = min(BN, a.cout - n0);
+
+  const fss_i32x4 rx = dma_resource(a.x + m0 * a.x_ld, kMmBytes);
+  const fss_i32x4 rw = dma_resource(a.w + (long long)n0 * a.w_ld, kMmBytes);
+  unsigned xoff[L::kXPieces], woff[L::kWPieces];
+  const int prow = lane >> 3, phys = lane & 7;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    v[e] = part[0][e][lane];
-#pragma unroll
-    for (int i = 1; i < kFewWaves; ++i) v[e] += part[i][e][lane];
+  for (int i = 0; i < L::kXPieces; ++i) {
+    const int row = (wave * L::kXPieces + i) * 8 + prow, chunk = phys ^ ((row >> 1) & 7);
+    xoff[i] = row < rows_left ? (unsigned)(row * (int)a.x_ld + chunk * 16) : kMmOutside + chunk * 16;
   }
-  finish8<T>(a, row, n0 + 8 * g, v);
+#pragma unroll
+  for (int i = 0; i < L::kWPieces; ++i) {
+    const int row = (wave * L::kWPieces + i) * 8 + prow, chunk = phys ^ ((row >> 1) & 7);
+    woff[i] = row < chans_left ? (unsigned)(row * (int)a.w_ld + chunk * 16) : kMmOutside + chunk * 16;
+  }
+  auto stage = [&](int kb, unsigned dst) {
+    const unsigned k0 = (unsigned)kb * 128u;
+    const bool whole = (int)k0 + 128 <= a.k, past = kb >= a.kblocks;            // uniform
+#pragma unroll
+    for (int i = 0; i < L::kXPieces; ++i) {
+      const int row = (wave * L::kXPieces + i) * 8 + prow, chunk = phys ^ ((row >> 1) & 7);
+      blds16(whole || (int)k0 + chunk * 16 < a.k ? xoff[i] + k0 : kMmOutside, rx,
+             dst + (wave * L::kXPieces + i) * 1024);
+    }
+#pragma unroll
+    for (int i = 0; i < L::kWPieces; ++i) {
+      const int row = (wave * L::kWPieces + i) * 8 + prow, chunk = phys ^ ((row >> 1) & 7);
+      blds16(whole || (int)k0 + chunk * 16 < a.k ? woff[i] + k0 : kMmOutside, rw,
+             dst + L::kXBytes + (wave * L::kWPieces + i) * 1024);
+    }
+    const unsigned sdst = dst + L::kXBytes + L::kWBytes + wave * 256;
+    if (wave < BM / 64) {
+      const fss_i32x4 rs = dma_resource(a.sx + kb * a.x_scale_ld + m0, past ? 0 : BM * 4);
+      const int row = wave * 64 + lane;
+      blds4(row < rows_left ? row * 4u : kMmOutside, rs, sdst);
+    } else if (wave == BM / 64) {
+      const fss_i32x4 rs = dma_resource(a.sw + kb * a.w_scale_ld + (n0 >> 7), past ? 0 : 1024);
+      blds4(lane * 128 < chans_left ? lane * 4u : kMmOutside, rs, sdst);
+    }
+  };
+
+  fss_f32x4 acc[TJ][TI];
+#pragma unroll
+  for (int j = 0; j < TJ; ++j)
+#pragma unroll
+    for (int i = 0; i < TI; ++i) acc[j][i] = fss_f32x4{0.f, 0.f, 0.f, 0.f};
+
+  const int r = lane & 15, g = lane >> 4;
+  const int xswz = (r >> 1) & 7;
+  const char* px = ring + (wm * TJ * 16 + r) * 128;
+  const char* psx = ring + L::kXBytes + L::kWBytes + (wm * TJ * 16 + r) * 4;
+  // weight rows of tile t of a pair: 8 (r / 4) + 4 t + r % 4
+  const int wrow0 = 8 * (r >> 2) + (r & 3), wswz0 = (wrow0 >> 1) & 7, wswz1 = ((wrow0 + 4) >> 1) & 7;
+  const char* pw = ring + L::kXBytes + (wn * TI * 16 + wrow0) * 128;
+  const char* psw = ring + L::kXBytes + L::kWBytes + BM * 4 + ((n0 & 127) + wn * TI * 16 >> 7) * 4;
+  const bool more = wave <= BM / 64;           // this wave copies scales, too
+
+  // blocks wk, wk + WK, ... of k; all groups make the same number of rounds (a round past the end of
+  // k deposits zeros), as they share the barriers
+  const int rounds = (a.kblocks + WK - 1) / WK;
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i)
+    if (i < rounds) stage(i * WK + wk, ring_base + i * L::kStage);
+  unsigned cur = 0, ahead = (NS - 1) * L::kStage;
+  for (int round = 0; round < rounds; ++round) {
+    // everything but the stages behind this one (those that exist) has landed
+    const int behind = rounds - 1 - round;
+    if (NS > 3 && behind >= 2) {
+      if (more) wait_vmcnt<(NS > 3 ? 2 : 0) * (L::kPieces + 1)>();
+      else wait_vmcnt<(NS > 3 ? 2 : 0) * L::kPieces>();
+    } else if (NS > 2 && behind >= 1) {
+      if (more) wait_vmcnt<(NS > 2 ? 1 : 0) * (L::kPieces + 1)>();
+      else wait_vmcnt<(NS > 2 ? 1 : 0) * L::kPieces>();
+    } else {
+      wait_vmcnt<0>();
+    }
+    __syncthreads();       // ... for every wave, and nobody reads the stage refilled next any more
+    if (round + NS - 1 < rounds) stage((round + NS - 1) * WK + wk, ring_base + ahead);
+    const float sw = *reinterpret_cast<const float*>(psw + cur);
+    Block<T> fw[TI];
+#pragma unroll
+    for (int i = 0; i < TI; ++i) {
+      const char* p = pw + cur + (i >> 1) * 32 * 128 + (i & 1) * 4 * 128;
+      const int swz = (i & 1) ? wswz1 : wswz0;
+      fw[i].set(*reinterpret_cast<const uint4*>(p + ((g ^ swz) << 4)),
+                *reinterpret_cast<const uint4*>(p + (((4 + g) ^ swz) << 4)));
+    }
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) {
+      Block<T> fx;
+      const char* p = px + cur + j * 16 * 128;
+      fx.set(*reinterpret_cast<const uint4*>(p + ((g ^ xswz) << 4)),
+             *reinterpret_cast<const uint4*>(p + (((4 + g) ^ xswz) << 4)));
+      const float s = sw * *reinterpret_cast<const float*>(psx + cur + j * 64);
+#pragma unroll
+      for (int i = 0; i < TI; ++i) {
+        const fss_f32x4 t = mma<T>(fw[i], fx);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[j][i][e] = fmaf(t[e], s, acc[j][i][e]);
+      }
+    }
+    cur = cur + L::kStage == NS * L::kStage ? 0 : cur + L::kStage;
+    ahead = ahead + L::kStage == NS * L::kStage ? 0 : ahead + L::kStage;
+  }
+
+  if constexpr (WK > 1) {
+    // the groups' sums are added in a fixed order; the rings are free after the barrier
+    static_assert(L::kLds >= (WK - 1) * L::kWaves * TJ * TI * 1024, "sums do not fit");
+    fss_f32x4* part = reinterpret_cast<fss_f32x4*>(smem) + (wave * TJ * TI) * 64 + lane;
+    constexpr int kGroup = L::kWaves * TJ * TI * 64;
+    __syncthreads();
+    if (wk > 0) {
+#pragma unroll
+      for (int j = 0; j < TJ; ++j)
+#pragma unroll
+        for (int i = 0; i < TI; ++i) part[(wk - 1) * kGroup + (j * TI + i) * 64] = acc[j][i];
+    }
+    __syncthreads();
+    if (wk > 0) return;
+#pragma unroll
+    for (int j = 0; j < TJ; ++j)
+#pragma unroll
+      for (int i = 0; i < TI; ++i)
+#pragma unroll
+        for (int z = 0; z < WK - 1; ++z) acc[j][i] += part[z * kGroup + (j * TI + i) * 64];
+  }
+  const Limits lim = limits_of<T>(a.act);
+#pragma unroll
+  for (int i = 0; i < TI; i += 2) {
+    const int c0 = (wn * TI + i) * 16 + 8 * g;
+    if (c0 >= chans_left) break;
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) {
+      const int row = (wm * TJ + j) * 16 + r;
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = acc[j][i][e];
+        v[4 + e] = acc[j][i + 1][e];
+      }
+      if (row < rows_left) finish8<T, VEC>(a, lim, m0 + row, n0 + c0, v);
+    }
+  }
+}
+
+template <typename T, bool VEC, int BM, int BN, int WM, int WN, int WK, int NS>
+int launch_tile(const MmArgs& a, hipStream_t stream) {
+  typedef MmTile<BM, BN, WM, WN, WK, NS> L;
+  const int tiles_n = ceil_div(a.cout, BN);
+  const long long tiles = (a.rows + BM - 1) / BM * tiles_n;
+  FSS_REQUIRE(tiles < 0x7fffffffLL, "too many tiles");
+  FSS_CHECK_HIP(hipFuncSetAttribute((const void*)matmul_fp8_tile_kernel<T, VEC, BM, BN, WM, WN, WK, NS>,
+                                    hipFuncAttributeMaxDynamicSharedMemorySize, L::kLds));
+  hipLaunchKernelGGL((matmul_fp8_tile_kernel<T, VEC, BM, BN, WM, WN, WK, NS>), dim3((unsigned)tiles), dim3(L::kThreads), L::kLds,
+                     stream, a, tiles_n);
+  FSS_LAUNCH_CHECK();
+  return 0;
+}
+
+template <typename T>
+int launch_few(const MmArgs& a, hipStream_t stream) {
+  const int chan_tiles = ceil_div(a.cout, 32);
+  const long long groups = (a.rows + 15) / 16 * chan_tiles;
+  FSS_REQUIRE(groups < 0x7fffffffLL, "too many tiles");
+  hipLaunchKernelGGL(matmul_fp8_few_kernel<T>, dim3((unsigned)groups), dim3(kFewWaves * 64), 0, stream, a, chan_tiles);
+  FSS_LAUNCH_CHECK();
+  return 0;
+}
+
+template <typename T>
+int launch_matmul(const MmArgs& a, hipStream_t stream) {
+  auto tiles = [&](int bm, int bn) { return (a.rows + bm - 1) / bm * ceil_div(a.cout, bn); };
+  // Rules measured over 1 to 132612 rows, 19 to 8192 channels and k from 128 to 8192 (us, 16-bit outputs):
+  //   few rows, while their work is at most 10 blocks of k per compute unit (1 x 512, k 2048: 5.0 against 7.6;
+  //   300 x 1024, k 1024: 8.0 against 6.1);
+  if ((a.rows + 15) / 16 * ceil_div(a.cout, 32) * a.kblocks <= 2560) return launch_few<T>(a, stream);
+#define FSS_TILE(...) \
+  return a.vec ? launch_tile<T, true, __VA_ARGS__>(a, stream) : launch_tile<T, false, __VA_ARGS__>(a, stream)
+  //   256 x 256 where they fill whole rounds of the 256 compute units and k is long enough to hide a tile's
+  //   ends (8192 x 8192, k 8192: 528 against 590; 33153 x 1024, k 2048, 2.03 rounds: 112 against 97);
+  const long long big = tiles(256, 256), rounds = (big + 255) / 256;
+  if (big >= 240 && big * 10 >= rounds * 256 * 9 && a.kblocks >= 8) FSS_TILE(256, 256, 2, 4, 1, 2);
+  //   128 x 128 from three per compute unit (33153 x 1024, k 2048: 97 against 115; 8385 x 1024, k 1024,
+  //   528 tiles: 24.0 against 21.7);
+  if (tiles(128, 128) >= 768) FSS_TILE(128, 128, 2, 2, 1, 2);
+  //   64 x 64 with two groups of waves along k where the chain of its blocks is what takes the time (2145 x
+  //   512, k 2048: 10.7 against 11.6; 8385 x 256, k 1024: 11.4 against 9.3), else with one.
+  if (tiles(64, 64) <= 512 && a.kblocks >= 8) FSS_TILE(64, 64, 2, 2, 2, 2);
+  FSS_TILE(64, 64, 2, 2, 1, 2);
+#undef FSS_TILE
 }
 
 int check_desc(const fss_matmul_fp8_desc* d) {
@@ -268,21 +523,13 @@ int fss_matmul_fp8(const fss_matmul_fp8_desc* desc, const void* x, const float* 
   a.rows = d.rows; a.x_ld = d.x_ld; a.x_scale_ld = d.x_scale_ld; a.w_ld = d.w_ld; a.w_scale_ld = d.w_scale_ld;
   a.res_ld = d.res_ld; a.y_ld = d.y_ld;
   a.cout = d.cout; a.k = d.k; a.kblocks = ceil_div(d.k, 128); a.act = d.act;
-  a.vec = (((uintptr_t)y | (uintptr_t)residual) & 15) == 0 && d.y_ld * es % 16 == 0 &&
+  a.vec = d.cout % 8 == 0 && (((uintptr_t)y | (uintptr_t)residual) & 15) == 0 && d.y_ld * es % 16 == 0 &&
           (residual == nullptr || d.res_ld * es % 16 == 0);
   hipStream_t s = (hipStream_t)stream;
-  const int chan_tiles = ceil_div(d.cout, 32);
-  const long long groups = (d.rows + 15) / 16 * chan_tiles;
-  FSS_REQUIRE(groups < 0x7fffffffLL, "too many tiles");
-#define FSS_MM(T) \
-  hipLaunchKernelGGL(matmul_fp8_few_kernel<T>, dim3((unsigned)groups), dim3(kFewWaves * 64), 0, s, a, chan_tiles)
-  if (d.out_dtype == FSS_F32) FSS_MM(float);
-  else if (d.out_dtype == FSS_BF16) FSS_MM(bf16_t);
-  else if (d.out_dtype == FSS_F16) FSS_MM(f16_t);
-  else FSS_MM(f32s_t);
-#undef FSS_MM
-  FSS_LAUNCH_CHECK();
-  return 0;
+  if (d.out_dtype == FSS_F32) return launch_matmul<float>(a, s);
+  if (d.out_dtype == FSS_BF16) return launch_matmul<bf16_t>(a, s);
+  if (d.out_dtype == FSS_F16) return launch_matmul<f16_t>(a, s);
+  return launch_matmul<f32s_t>(a, s);
 }
 
 }  // extern "C"
