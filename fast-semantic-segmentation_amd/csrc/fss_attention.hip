@@ -116,24 +116,67 @@ attention_kernel(const AttnArgs a) {
   for (int i = 0; i < DP / 32; ++i) o[i] = f32x16_t{};
   float m = -INFINITY, l = 0.f;
 
-  for (int tile = tile0; tile < tile1; ++tile) {
+  // pieces of a tile this wave copies: byte offsets from the tile's first key, which only the last tile
+  // checks against the length
+  constexpr int kMine = L::kPieces / NW;
+  static_assert(L::kPieces % NW == 0, "pieces per wave");
+  unsigned koff[kMine], voff[kMine];
+  int prow[kMine];
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int at = (wave * kMine + i) * 64 + lane, row = at / L::kChunks, phys = at % L::kChunks;
+    const int ck = phys ^ L::kswz(row), cv = phys ^ L::vswz(row);
+    prow[i] = row;
+    koff[i] = ck * 8 < a.d ? (unsigned)(row * 2 * (int)a.ks[1] + ck * 16) : kDmaOutOfRange;
+    voff[i] = cv * 8 < a.d ? (unsigned)(row * 2 * (int)a.vs[1] + cv * 16) : kDmaOutOfRange;
+  }
+  // copies a tile to buffer 0 or 1: keys at or behind the length and channels behind head_dim are zeros
+  auto stage = [&](int tile, unsigned dst) {
     const int key0 = tile * kKeys, left = len - key0;
-    // copy the tile: keys at or behind the length and channels behind head_dim are filled with zeros
-    __syncthreads();
-    {
-      const fss_i32x4 rk = dma_resource(kbase + 2 * (long long)key0 * a.ks[1], ~0ull);
-      const fss_i32x4 rv = dma_resource(vbase + 2 * (long long)key0 * a.vs[1], ~0ull);
-      for (int p = wave; p < L::kPieces; p += NW) {
-        const int at = p * 64 + lane, row = at / L::kChunks, phys = at % L::kChunks;
-        const int ck = phys ^ L::kswz(row), cv = phys ^ L::vswz(row);
-        blds16(row < left && ck * 8 < a.d ? (unsigned)(row * 2 * (int)a.ks[1] + ck * 16) : kDmaOutOfRange, rk,
-               smem_base + p * 1024);
-        blds16(row < left && cv * 8 < a.d ? (unsigned)(row * 2 * (int)a.vs[1] + cv * 16) : kDmaOutOfRange, rv,
-               smem_base + L::kBytes + p * 1024);
+    const fss_i32x4 rk = dma_resource(kbase + 2 * (long long)key0 * a.ks[1], ~0ull);
+    const fss_i32x4 rv = dma_resource(vbase + 2 * (long long)key0 * a.vs[1], ~0ull);
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const bool in = prow[i] < left;
+      blds16(in ? koff[i] : kDmaOutOfRange, rk, dst + (wave * kMine + i) * 1024);
+      blds16(in ? voff[i] : kDmaOutOfRange, rv, dst + L::kBytes + (wave * kMine + i) * 1024);
+    }
+  };
+  // mask of a tile: this lane reads 32 consecutive keys (those of score tile h) of its query
+  uint4 mnext[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+  auto mask_ahead = [&](int tile) {
+    const int key0 = tile * kKeys;
+    if (key0 + kKeys <= len) {
+      typedef uint4 loose __attribute__((aligned(1)));
+      mnext[0] = *reinterpret_cast<const loose*>(mp + key0 + 32 * h);
+      mnext[1] = *reinterpret_cast<const loose*>(mp + key0 + 32 * h + 16);
+    }
+  };
+
+  if constexpr (MASK) {
+    if (tile0 < tile1) mask_ahead(tile0);
+  }
+  if (tile0 < tile1) stage(tile0, smem_base);
+  unsigned cur = 0;
+  for (int tile = tile0; tile < tile1; ++tile, cur ^= 2 * L::kBytes) {
+    const int key0 = tile * kKeys, left = len - key0;
+    wait_vmcnt<0>();
+    __syncthreads();     // the tile has landed for every wave, and nobody reads the other buffer any more
+    // mask dwords, 4 keys each: own keys of score tile 0 and 1, exchanged with lane + 32
+    unsigned md[2][4];
+    if constexpr (MASK) {
+      const unsigned w[8] = {mnext[0].x, mnext[0].y, mnext[0].z, mnext[0].w, mnext[1].x, mnext[1].y, mnext[1].z, mnext[1].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const auto t = __builtin_amdgcn_permlane32_swap(w[2 * j], w[2 * j + 1], false, false);
+        md[0][j] = t[0];
+        md[1][j] = t[1];
       }
     }
-    wait_vmcnt<0>();
-    __syncthreads();
+    if (tile + 1 < tile1) {
+      if constexpr (MASK) mask_ahead(tile + 1);
+      stage(tile + 1, smem_base + (cur ^ (2 * L::kBytes)));
+    }
 
     // scores of 64 keys
     f32x16_t s[2];
@@ -141,12 +184,12 @@ attention_kernel(const AttnArgs a) {
     for (int kt = 0; kt < 2; ++kt) {
       s[kt] = f32x16_t{};
       const int row = kt * 32 + col;
-      const char* base = smem + row * L::kRow;
+      const char* base = smem + cur + row * L::kRow;
 #pragma unroll
       for (int st = 0; st < DP / 16; ++st)
         s[kt] = mfma32<T>(*reinterpret_cast<const uint4*>(base + ((2 * st + h) ^ L::kswz(row)) * 16), qf[st], s[kt]);
     }
-    if (left < kKeys || MASK) {
+    if (left < kKeys) {
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -156,6 +199,12 @@ attention_kernel(const AttnArgs a) {
           if constexpr (MASK) seen = seen && mp[seen ? key0 + key : 0] != 0;
           s[kt][i] = seen ? s[kt][i] : -INFINITY;
         }
+    } else if constexpr (MASK) {
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          s[kt][i] = (md[kt][i / 4] >> (8 * (i % 4)) & 0xffu) != 0 ? s[kt][i] : -INFINITY;
     }
     float top = -INFINITY;
 #pragma unroll
@@ -163,12 +212,16 @@ attention_kernel(const AttnArgs a) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kt][i]);
     top = other_half_max(top) * a.c;
-    const float m_new = fmaxf(m, top), m_use = m_new == -INFINITY ? 0.f : m_new;
-    const float alpha = __builtin_amdgcn_exp2f(m - m_use);
-    m = m_new;
-    l *= alpha;
+    // the sums are rescaled only where some query's maximum has grown (after a few tiles, hardly ever)
+    if (__any(top > m)) {
+      const float m_new = fmaxf(m, top);
+      const float alpha = __builtin_amdgcn_exp2f(m - (m_new == -INFINITY ? 0.f : m_new));
+      m = m_new;
+      l *= alpha;
 #pragma unroll
-    for (int i = 0; i < DP / 32; ++i) o[i] *= alpha;
+      for (int i = 0; i < DP / 32; ++i) o[i] *= alpha;
+    }
+    const float m_use = m == -INFINITY ? 0.f : m;
     unsigned pf[2][8];
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
@@ -192,7 +245,8 @@ attention_kernel(const AttnArgs a) {
         for (int j = 0; j < 2; ++j) {
           const int key = ks * 16 + j * 8 + 4 * (g16 >> 1) + (i16 >> 2);
           const int byte = dt * 64 + (g16 & 1) * 32 + (i16 & 3) * 8;
-          const unsigned at = smem_base + L::kBytes + key * L::kRow + (((byte >> 4) ^ L::vswz(key)) << 4) + (byte & 8);
+          const unsigned at =
+              smem_base + cur + L::kBytes + key * L::kRow + (((byte >> 4) ^ L::vswz(key)) << 4) + (byte & 8);
           half[j] = __builtin_bit_cast(
               uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                          (__attribute__((address_space(3))) i16x4_t*)(__attribute__((address_space(3))) char*)(size_t)at));
@@ -203,7 +257,7 @@ attention_kernel(const AttnArgs a) {
   }
 
   l += __shfl_xor(l, 32);
-  const long long prow = ((long long)z * a.batch * a.kv_heads + bh) * a.rows + r;
+  const long long part = ((long long)z * a.batch * a.kv_heads + bh) * a.rows + r;
   const float f = SPLIT ? 1.f : l > 0.f ? 1.f / l : (l == l ? 0.f : l);
   char* yp = a.y + 2 * (b * a.ys[0] + token * a.ys[1] + head * a.ys[2]);
 
@@ -262,8 +316,8 @@ attention_kernel(const AttnArgs a) {
   if (!row_ok) return;
   if constexpr (SPLIT) {
     if (h == 0) {
-      a.part_ml[prow * 2] = m;
-      a.part_ml[prow * 2 + 1] = l;
+      a.part_ml[part * 2] = m;
+      a.part_ml[part * 2 + 1] = l;
     }
   }
   if (done) return;
@@ -275,7 +329,7 @@ attention_kernel(const AttnArgs a) {
       if (ch >= a.d) continue;
       const float v0 = o[dt][4 * j], v1 = o[dt][4 * j + 1], v2 = o[dt][4 * j + 2], v3 = o[dt][4 * j + 3];
       if constexpr (SPLIT)
-        *reinterpret_cast<float4*>(a.part_o + prow * a.d + ch) = make_float4(v0, v1, v2, v3);
+        *reinterpret_cast<float4*>(a.part_o + part * a.d + ch) = make_float4(v0, v1, v2, v3);
       else
         *reinterpret_cast<uint2*>(yp + ch * 2) =
             l == 0.f ? make_uint2(0, 0) : make_uint2(pack2_sat<T>(v0 * f, v1 * f), pack2_sat<T>(v2 * f, v3 * f));
@@ -353,7 +407,7 @@ size_t workspace_of(const fss_attention_desc& d, const Shape& s) {
 template <typename T, int DP, int NW>
 int launch(const AttnArgs& a, const Shape& s, hipStream_t stream) {
   const dim3 grid((unsigned)((long long)a.batch * a.kv_heads * a.qtiles * a.splits));
-  const size_t lds = 2 * Tile<DP>::kBytes;
+  const size_t lds = 4 * Tile<DP>::kBytes;
 #define FSS_ATTN(MASK, SPLIT)                                                                                       \
   do {                                                                                                              \
     FSS_CHECK_HIP(hipFuncSetAttribute((const void*)attention_kernel<T, DP, NW, MASK, SPLIT>,                        \
