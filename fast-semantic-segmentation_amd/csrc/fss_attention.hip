@@ -68,7 +68,7 @@ template <typename T> __device__ __forceinline__ unsigned pack2_sat(float a, flo
 }
 
 template <typename T, int DP, int NW, bool MASK, bool SPLIT>
-__global__ void __launch_bounds__(NW * 64)
+__global__ void __launch_bounds__(NW * 64, DP <= 64 ? 3 : DP <= 128 ? 2 : 1)
 attention_kernel(const AttnArgs a) {
   typedef Tile<DP> L;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
@@ -116,30 +116,28 @@ attention_kernel(const AttnArgs a) {
   for (int i = 0; i < DP / 32; ++i) o[i] = f32x16_t{};
   float m = -INFINITY, l = 0.f;
 
-  // pieces of a tile this wave copies: byte offsets from the tile's first key, which only the last tile
-  // checks against the length
-  constexpr int kMine = L::kPieces / NW;
+  // copies a tile to a buffer, 1 KiB pieces dealt to the waves: keys at or behind the length and channels
+  // behind head_dim are zeros.  The XOR of a row is the XOR of its piece's first row and of the
+  // lane's row in the piece (they share no bits), so a piece costs few instructions and no registers.
+  constexpr int kMine = L::kPieces / NW, kRows = 64 / L::kChunks;
   static_assert(L::kPieces % NW == 0, "pieces per wave");
-  unsigned koff[kMine], voff[kMine];
-  int prow[kMine];
-#pragma unroll
-  for (int i = 0; i < kMine; ++i) {
-    const int at = (wave * kMine + i) * 64 + lane, row = at / L::kChunks, phys = at % L::kChunks;
-    const int ck = phys ^ L::kswz(row), cv = phys ^ L::vswz(row);
-    prow[i] = row;
-    koff[i] = ck * 8 < a.d ? (unsigned)(row * 2 * (int)a.ks[1] + ck * 16) : kDmaOutOfRange;
-    voff[i] = cv * 8 < a.d ? (unsigned)(row * 2 * (int)a.vs[1] + cv * 16) : kDmaOutOfRange;
-  }
-  // copies a tile to buffer 0 or 1: keys at or behind the length and channels behind head_dim are zeros
+  const int lrow = lane / L::kChunks;
+  const int ck0 = lane % L::kChunks ^ L::kswz(lrow), cv0 = lane % L::kChunks ^ L::vswz(lrow);
+  const unsigned klane = lrow * 2 * (unsigned)a.ks[1], vlane = lrow * 2 * (unsigned)a.vs[1];
+  const bool full = a.d == DP;
   auto stage = [&](int tile, unsigned dst) {
-    const int key0 = tile * kKeys, left = len - key0;
+    const int key0 = tile * kKeys, left = len - key0 - lrow;
     const fss_i32x4 rk = dma_resource(kbase + 2 * (long long)key0 * a.ks[1], ~0ull);
     const fss_i32x4 rv = dma_resource(vbase + 2 * (long long)key0 * a.vs[1], ~0ull);
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
-      const bool in = prow[i] < left;
-      blds16(in ? koff[i] : kDmaOutOfRange, rk, dst + (wave * kMine + i) * 1024);
-      blds16(in ? voff[i] : kDmaOutOfRange, rv, dst + L::kBytes + (wave * kMine + i) * 1024);
+      const int piece = wave * kMine + i, row0 = piece * kRows;
+      const int ck = ck0 ^ L::kswz(row0), cv = cv0 ^ L::vswz(row0);
+      const bool in = row0 < left;
+      blds16(in && (full || ck * 8 < a.d) ? klane + row0 * 2 * (unsigned)a.ks[1] + ck * 16 : kDmaOutOfRange, rk,
+             dst + piece * 1024);
+      blds16(in && (full || cv * 8 < a.d) ? vlane + row0 * 2 * (unsigned)a.vs[1] + cv * 16 : kDmaOutOfRange, rv,
+             dst + L::kBytes + piece * 1024);
     }
   };
   // mask of a tile: this lane reads 32 consecutive keys (those of score tile h) of its query
