@@ -20,6 +20,7 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kKeys = 64;              // keys per tile
+constexpr int kMfma = 0x8, kDsRead = 0x100, kValu = 0x402;     // instruction classes of sched_group_barrier
 
 struct AttnArgs {
   const char* q;
@@ -57,7 +58,17 @@ template <int DP> struct Tile {
   }
 };
 
-__device__ __forceinline__ float other_half_max(float v) { return fmaxf(v, __shfl_xor(v, 32)); }
+// largest of lanes l and l + 32, in both
+__device__ __forceinline__ float other_half_max(float v) {
+  const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
+}
+
+typedef __attribute__((address_space(3))) const char* lds_ptr;
+typedef __attribute__((address_space(3))) i16x4_t* lds_tr_ptr;
+__device__ __forceinline__ uint4 lds16(lds_ptr p) {
+  return __builtin_bit_cast(uint4, *(const __attribute__((address_space(3))) fss_u32x4*)p);
+}
 
 template <typename T> __device__ __forceinline__ unsigned pack2_sat(float a, float b) {
   if constexpr (__is_same(T, f16_t)) {
@@ -76,11 +87,10 @@ attention_kernel(const AttnArgs a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, h = lane >> 5;
 
-  // blocks that share keys and values are neighbours on one XCD (its L2 holds them)
-  const int nwg = gridDim.x, bid = blockIdx.x;
-  const int q8 = nwg >> 3, rr = nwg & 7, xcd = bid & 7;
-  const int wg = (xcd < rr ? xcd * (q8 + 1) : rr * (q8 + 1) + (xcd - rr) * q8) + (bid >> 3);
-  const int qt = wg % a.qtiles, rest = wg / a.qtiles;
+  // Query tiles of one head follow each other and so run at about the same time, spread over all XCDs: each
+  // XCD's L2 holds the keys and values once, and batch entries of different length load all XCDs alike
+  // (one head per XCD instead: 1.23 against 1.12 ms for 2 x 16 heads, 8385 queries, 8385 and 6288 keys).
+  const int qt = blockIdx.x % a.qtiles, rest = blockIdx.x / a.qtiles;
   const int z = rest % a.splits, bh = rest / a.splits;
   const int b = bh / a.kv_heads, hk = bh % a.kv_heads;
 
@@ -151,6 +161,20 @@ attention_kernel(const AttnArgs a) {
     }
   };
 
+  // Transposing reads of V: each group of 16 lanes takes 4 keys x 16 channels.  The row XOR depends on the
+  // lane alone and moves 64-byte pieces among 4 (2, 1 for short rows), hence one base per piece.
+  constexpr int kVBases = L::kChunks < 16 ? L::kChunks / 4 : 4;
+  lds_ptr vfrag[kVBases];
+  {
+    const int key = 4 * (lane >> 5) + ((lane & 15) >> 2), in64 = (lane >> 4 & 1) * 32 + (lane & 3) * 8;
+#pragma unroll
+    for (int i = 0; i < kVBases; ++i)
+      vfrag[i] = (lds_ptr)smem + L::kBytes + key * L::kRow + ((i * 4 ^ L::vswz(key)) << 4) + in64;
+  }
+  lds_ptr kfrag[DP / 16];
+#pragma unroll
+  for (int st = 0; st < DP / 16; ++st) kfrag[st] = (lds_ptr)smem + col * L::kRow + (((2 * st + h) ^ L::kswz(col)) << 4);
+
   if constexpr (MASK) {
     if (tile0 < tile1) mask_ahead(tile0);
   }
@@ -178,16 +202,23 @@ attention_kernel(const AttnArgs a) {
 
     // scores of 64 keys
     f32x16_t s[2];
+    s[0] = f32x16_t{};
+    s[1] = f32x16_t{};
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      s[kt] = f32x16_t{};
-      const int row = kt * 32 + col;
-      const char* base = smem + cur + row * L::kRow;
+    for (int st = 0; st < DP / 16; ++st)
 #pragma unroll
-      for (int st = 0; st < DP / 16; ++st)
-        s[kt] = mfma32<T>(*reinterpret_cast<const uint4*>(base + ((2 * st + h) ^ L::kswz(row)) * 16), qf[st], s[kt]);
+      for (int kt = 0; kt < 2; ++kt)
+        s[kt] = mfma32<T>(lds16(kfrag[st] + cur + kt * 32 * L::kRow), qf[st], s[kt]);
+    // issue order: reads four ahead of the products that take them
+    __builtin_amdgcn_sched_group_barrier(kDsRead, 4, 0);
+#pragma unroll
+    for (int i = 0; i < DP / 8 - 4; ++i) {
+      __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
     }
+    __builtin_amdgcn_sched_group_barrier(kMfma, 4, 0);
     if (left < kKeys) {
+      asm volatile("");      // keeps the comparisons below out of the path of whole tiles
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -230,27 +261,34 @@ attention_kernel(const AttnArgs a) {
         l += p0 + p1;
         pf[kt][i] = Half16<T>::pack2(p0, p1);
       }
-    // O^T += V^T P^T, 16 keys at a time; lane group of 16: 4 keys x 16 channels, transposed on the way
-    const int g16 = lane >> 4, i16 = lane & 15;
+    // O^T += V^T P^T, 16 keys at a time
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
       const uint4 pb = make_uint4(pf[ks / 2][4 * (ks & 1)], pf[ks / 2][4 * (ks & 1) + 1], pf[ks / 2][4 * (ks & 1) + 2],
                                   pf[ks / 2][4 * (ks & 1) + 3]);
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt) {
-        uint2 half[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int key = ks * 16 + j * 8 + 4 * (g16 >> 1) + (i16 >> 2);
-          const int byte = dt * 64 + (g16 & 1) * 32 + (i16 & 3) * 8;
-          const unsigned at =
-              smem_base + cur + L::kBytes + key * L::kRow + (((byte >> 4) ^ L::vswz(key)) << 4) + (byte & 8);
-          half[j] = __builtin_bit_cast(
-              uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                         (__attribute__((address_space(3))) i16x4_t*)(__attribute__((address_space(3))) char*)(size_t)at));
-        }
-        o[dt] = mfma32<T>(make_uint4(half[0].x, half[0].y, half[1].x, half[1].y), pb, o[dt]);
+        const lds_ptr at = vfrag[dt % kVBases] + cur + (dt / kVBases) * kVBases * 64 + ks * 16 * L::kRow;
+        const uint2 v0 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)at));
+        const uint2 v1 =
+            __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(at + 8 * L::kRow)));
+        o[dt] = mfma32<T>(make_uint4(v0.x, v0.y, v1.x, v1.y), pb, o[dt]);
       }
+    }
+    // issue order: the exponentials of the second 32 keys between the products of the first
+    constexpr int kHalf = DP / 16;                    // products per 32 keys
+    __builtin_amdgcn_sched_group_barrier(kDsRead, 4, 1);
+    __builtin_amdgcn_sched_group_barrier(kValu, 56, 1);
+#pragma unroll
+    for (int i = 0; i < kHalf; ++i) {
+      __builtin_amdgcn_sched_group_barrier(kMfma, 1, 1);
+      __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 1);
+      __builtin_amdgcn_sched_group_barrier(kValu, 56 / kHalf, 1);
+    }
+#pragma unroll
+    for (int i = 0; i < kHalf; ++i) {
+      __builtin_amdgcn_sched_group_barrier(kMfma, 1, 1);
+      __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 1);
     }
   }
 
