@@ -58,6 +58,17 @@ template <int DP> struct Tile {
   }
 };
 
+// sum + both values of a pair, in float (one v_dot2): the rounded p, as the product with v takes them, so
+// that their errors partly cancel in the quotient
+template <typename T> __device__ __forceinline__ float add_pair(unsigned pair, float sum) {
+  if constexpr (__is_same(T, f16_t))
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(fss_f16x2, pair), __builtin_bit_cast(fss_f16x2, Half16<T>::kOnePair),
+                                  sum, false);
+  else
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(fss_bf16x2, pair),
+                                           __builtin_bit_cast(fss_bf16x2, Half16<T>::kOnePair), sum, false);
+}
+
 // largest of lanes l and l + 32, in both
 __device__ __forceinline__ float other_half_max(float v) {
   const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -76,6 +87,22 @@ template <typename T> __device__ __forceinline__ unsigned pack2_sat(float a, flo
     b = b > 65504.f ? 65504.f : b < -65504.f ? -65504.f : b;
   }
   return Half16<T>::pack2(a, b);
+}
+
+// Buffers of a tile: as many as leave LDS for three (head_dim above 64: two) workgroups of four waves per
+// compute unit; two where mask loads share the counter that the copies are waited for with.
+template <int DP, bool MASK> constexpr int kStages = MASK || DP > 64 ? 2 : DP > 32 ? 3 : 4;
+
+// blds16 with a wave-uniform byte offset besides the per-lane one (which alone is checked against the
+// buffer's end, less soff)
+__device__ __forceinline__ void blds16_at(unsigned voff, fss_i32x4 rsrc, unsigned soff, unsigned lds_dst) {
+  asm volatile(
+      "s_mov_b32 m0, %3\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %0, %1, %2 offen lds"
+      :
+      : "v"(voff), "s"(rsrc), "s"(soff), "s"(lds_dst)
+      : "memory", "m0");
 }
 
 template <typename T, int DP, int NW, bool MASK, bool SPLIT>
@@ -128,26 +155,42 @@ attention_kernel(const AttnArgs a) {
 
   // copies a tile to a buffer, 1 KiB pieces dealt to the waves: keys at or behind the length and channels
   // behind head_dim are zeros.  The XOR of a row is the XOR of its piece's first row and of the
-  // lane's row in the piece (they share no bits), so a piece costs few instructions and no registers.
+  // lane's row in the piece (they share no bits), and the former takes few values per wave.
   constexpr int kMine = L::kPieces / NW, kRows = 64 / L::kChunks;
-  static_assert(L::kPieces % NW == 0, "pieces per wave");
+  constexpr int kKPat = DP / 32 / NW > 0 ? DP / 32 / NW : 1, kVPat = DP == 256 && NW == 1 ? 2 : 1;
+  static_assert(L::kPieces % NW == 0 && kMine % kKPat == 0, "pieces per wave");
   const int lrow = lane / L::kChunks;
-  const int ck0 = lane % L::kChunks ^ L::kswz(lrow), cv0 = lane % L::kChunks ^ L::vswz(lrow);
-  const unsigned klane = lrow * 2 * (unsigned)a.ks[1], vlane = lrow * 2 * (unsigned)a.vs[1];
-  const bool full = a.d == DP;
+  unsigned koff[kKPat], voff[kVPat];
+#pragma unroll
+  for (int i = 0; i < kKPat; ++i) {
+    const int c = lane % L::kChunks ^ L::kswz(lrow) ^ L::kswz((i * NW + wave) * kRows);
+    koff[i] = c * 8 < a.d ? lrow * 2 * (unsigned)a.ks[1] + c * 16 : kDmaOutOfRange;
+  }
+#pragma unroll
+  for (int i = 0; i < kVPat; ++i) {
+    const int c = lane % L::kChunks ^ L::vswz(lrow) ^ L::vswz((i * NW + wave) * kRows);
+    voff[i] = c * 8 < a.d ? lrow * 2 * (unsigned)a.vs[1] + c * 16 : kDmaOutOfRange;
+  }
   auto stage = [&](int tile, unsigned dst) {
-    const int key0 = tile * kKeys, left = len - key0 - lrow;
+    const int key0 = tile * kKeys, left = len - key0;
     const fss_i32x4 rk = dma_resource(kbase + 2 * (long long)key0 * a.ks[1], ~0ull);
     const fss_i32x4 rv = dma_resource(vbase + 2 * (long long)key0 * a.vs[1], ~0ull);
+    if (left >= kKeys) {
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-      const int piece = wave * kMine + i, row0 = piece * kRows;
-      const int ck = ck0 ^ L::kswz(row0), cv = cv0 ^ L::vswz(row0);
-      const bool in = row0 < left;
-      blds16(in && (full || ck * 8 < a.d) ? klane + row0 * 2 * (unsigned)a.ks[1] + ck * 16 : kDmaOutOfRange, rk,
-             dst + piece * 1024);
-      blds16(in && (full || cv * 8 < a.d) ? vlane + row0 * 2 * (unsigned)a.vs[1] + cv * 16 : kDmaOutOfRange, rv,
-             dst + L::kBytes + piece * 1024);
+      for (int i = 0; i < kMine; ++i) {
+        const int piece = i * NW + wave, row0 = piece * kRows;
+        blds16_at(koff[i % kKPat], rk, row0 * 2 * (unsigned)a.ks[1], dst + piece * 1024);
+        blds16_at(voff[i % kVPat], rv, row0 * 2 * (unsigned)a.vs[1], dst + L::kBytes + piece * 1024);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int piece = i * NW + wave, row0 = piece * kRows;
+        const bool in = lrow + row0 < left;
+        blds16_at(in ? koff[i % kKPat] : kDmaOutOfRange, rk, row0 * 2 * (unsigned)a.ks[1], dst + piece * 1024);
+        blds16_at(in ? voff[i % kVPat] : kDmaOutOfRange, rv, row0 * 2 * (unsigned)a.vs[1],
+                  dst + L::kBytes + piece * 1024);
+      }
     }
   };
   // mask of a tile: this lane reads 32 consecutive keys (those of score tile h) of its query
@@ -178,12 +221,19 @@ attention_kernel(const AttnArgs a) {
   if constexpr (MASK) {
     if (tile0 < tile1) mask_ahead(tile0);
   }
-  if (tile0 < tile1) stage(tile0, smem_base);
-  unsigned cur = 0;
-  for (int tile = tile0; tile < tile1; ++tile, cur ^= 2 * L::kBytes) {
+  constexpr int NS = kStages<DP, MASK>, kTile = 2 * L::kBytes;
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i)
+    if (tile0 + i < tile1) stage(tile0 + i, smem_base + i * kTile);
+  unsigned cur = 0, ahead = (NS - 1) * kTile;
+  for (int tile = tile0; tile < tile1; ++tile) {
     const int key0 = tile * kKeys, left = len - key0;
-    wait_vmcnt<0>();
-    __syncthreads();     // the tile has landed for every wave, and nobody reads the other buffer any more
+    // everything but the tiles behind this one (those that exist) has landed
+    const int behind = tile1 - 1 - tile;
+    if (NS > 3 && behind >= 2) wait_vmcnt<(NS > 3 ? 4 * kMine : 0)>();
+    else if (NS > 2 && behind >= 1) wait_vmcnt<(NS > 2 ? 2 * kMine : 0)>();
+    else wait_vmcnt<0>();
+    __syncthreads();     // ... for every wave, and nobody reads the buffer refilled next any more
     // mask dwords, 4 keys each: own keys of score tile 0 and 1, exchanged with lane + 32
     unsigned md[2][4];
     if constexpr (MASK) {
@@ -195,10 +245,10 @@ attention_kernel(const AttnArgs a) {
         md[1][j] = t[1];
       }
     }
-    if (tile + 1 < tile1) {
-      if constexpr (MASK) mask_ahead(tile + 1);
-      stage(tile + 1, smem_base + (cur ^ (2 * L::kBytes)));
+    if constexpr (MASK) {
+      if (tile + 1 < tile1) mask_ahead(tile + 1);
     }
+    if (tile + NS - 1 < tile1) stage(tile + NS - 1, smem_base + ahead);
 
     // scores of 64 keys
     f32x16_t s[2];
@@ -258,8 +308,8 @@ attention_kernel(const AttnArgs a) {
       for (int i = 0; i < 8; ++i) {
         const float p0 = __builtin_amdgcn_exp2f(fmaf(s[kt][2 * i], a.c, -m_use));
         const float p1 = __builtin_amdgcn_exp2f(fmaf(s[kt][2 * i + 1], a.c, -m_use));
-        l += p0 + p1;
         pf[kt][i] = Half16<T>::pack2(p0, p1);
+        l = add_pair<T>(pf[kt][i], l);
       }
     // O^T += V^T P^T, 16 keys at a time
 #pragma unroll
@@ -278,18 +328,20 @@ attention_kernel(const AttnArgs a) {
     // issue order: the exponentials of the second 32 keys between the products of the first
     constexpr int kHalf = DP / 16;                    // products per 32 keys
     __builtin_amdgcn_sched_group_barrier(kDsRead, 4, 1);
-    __builtin_amdgcn_sched_group_barrier(kValu, 56, 1);
+    __builtin_amdgcn_sched_group_barrier(kValu, 48, 1);
 #pragma unroll
     for (int i = 0; i < kHalf; ++i) {
       __builtin_amdgcn_sched_group_barrier(kMfma, 1, 1);
       __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 1);
-      __builtin_amdgcn_sched_group_barrier(kValu, 56 / kHalf, 1);
+      __builtin_amdgcn_sched_group_barrier(kValu, 48 / kHalf, 1);
     }
 #pragma unroll
     for (int i = 0; i < kHalf; ++i) {
       __builtin_amdgcn_sched_group_barrier(kMfma, 1, 1);
       __builtin_amdgcn_sched_group_barrier(kDsRead, 2, 1);
     }
+    cur = cur + kTile == NS * kTile ? 0 : cur + kTile;
+    ahead = ahead + kTile == NS * kTile ? 0 : ahead + kTile;
   }
 
   l += __shfl_xor(l, 32);
@@ -372,50 +424,113 @@ attention_kernel(const AttnArgs a) {
     }
 }
 
-// Joins the pieces of the key axis: weights 2^(m_z - max m), in index order.  One thread per 4 channels.
+// y of a row's 4 channels from their joined sums
 template <typename T>
-__global__ void __launch_bounds__(256) attention_join_kernel(const AttnArgs a, long long all_rows) {
-  const int quads = a.d / 4;
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  const long long row = i / quads;
-  if (row >= all_rows) return;
-  const int ch = (int)(i % quads) * 4;
-  float top = -INFINITY;
-  for (int z = 0; z < a.splits; ++z) top = fmaxf(top, a.part_ml[(z * all_rows + row) * 2]);
-  if (top == -INFINITY) top = 0.f;
-  float l = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int z = 0; z < a.splits; ++z) {
-    const float* ml = a.part_ml + (z * all_rows + row) * 2;
-    const float w = __builtin_amdgcn_exp2f(ml[0] - top);
-    const float4 t = *reinterpret_cast<const float4*>(a.part_o + (z * all_rows + row) * a.d + ch);
-    if (ml[1] == 0.f) continue;          // this piece holds no key of the query
-    l = fmaf(w, ml[1], l);
-    v[0] = fmaf(w, t.x, v[0]); v[1] = fmaf(w, t.y, v[1]); v[2] = fmaf(w, t.z, v[2]); v[3] = fmaf(w, t.w, v[3]);
-  }
-  const long long bh = row / a.rows;
-  const int r = (int)(row % a.rows);
-  const int b = (int)(bh / a.kv_heads), head = (int)(bh % a.kv_heads) * a.group + r % a.group;
+__device__ __forceinline__ void store_joined(const AttnArgs& a, int row, int ch, const float4& v, float l) {
+  const int bh = row / a.rows, r = row - bh * a.rows;
+  const int b = bh / a.kv_heads, head = (bh - b * a.kv_heads) * a.group + r % a.group;
   const float f = l == 0.f ? 0.f : 1.f / l;
   *reinterpret_cast<uint2*>(a.y + 2 * (b * a.ys[0] + r / a.group * a.ys[1] + head * a.ys[2] + ch)) =
-      make_uint2(pack2_sat<T>(v[0] * f, v[1] * f), pack2_sat<T>(v[2] * f, v[3] * f));
+      make_uint2(pack2_sat<T>(v.x * f, v.y * f), pack2_sat<T>(v.z * f, v.w * f));
+}
+__device__ __forceinline__ void add_piece(float4& v, float w, const float4& o) {
+  if (w != 0.f) v = make_float4(fmaf(w, o.x, v.x), fmaf(w, o.y, v.y), fmaf(w, o.z, v.z), fmaf(w, o.w, v.w));
+}
+
+// Joins few pieces of the key axis, weights 2^(m_z - max m), in index order: one thread per 4 channels.
+constexpr int kFewSplits = 8;
+
+template <typename T>
+__global__ void __launch_bounds__(256) attention_join_few_kernel(const AttnArgs a, long long all_rows) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int quads = a.d / 4;
+  const long long row = i / quads;
+  if (row >= all_rows) return;
+  const int ch = (int)(i - row * quads) * 4;
+  float2 ml[kFewSplits];
+  float4 o[kFewSplits];
+  float top = -INFINITY;
+#pragma unroll
+  for (int z = 0; z < kFewSplits; ++z) {
+    const long long at = (long long)min(z, a.splits - 1) * all_rows + row;
+    ml[z] = reinterpret_cast<const float2*>(a.part_ml)[at];
+    o[z] = *reinterpret_cast<const float4*>(a.part_o + at * a.d + ch);
+    top = fmaxf(top, ml[z].x);
+  }
+  float l = 0.f;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int z = 0; z < kFewSplits; ++z) {
+    const float w = z >= a.splits || ml[z].y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml[z].x - top);
+    if (w != 0.f) l = fmaf(w, ml[z].y, l);
+    add_piece(v, w, o[z]);
+  }
+  store_joined<T>(a, (int)row, ch, v, l);
+}
+
+// Joins many pieces: one row per workgroup; thread z forms the weight of piece z, then QP threads of 4
+// channels x 256 / QP groups of pieces add them, all loads of a row in flight at once (a serial walk over 34
+// pieces took 10 us), in a fixed order.
+constexpr int kMaxSplits = 256;
+
+template <typename T, int QP>
+__global__ void __launch_bounds__(256) attention_join_kernel(const AttnArgs a, int all_rows) {
+  constexpr int G = 256 / QP;
+  __shared__ float weight[kMaxSplits], red[8];
+  __shared__ float4 sums[256];
+  const int row = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  float2 ml = make_float2(-INFINITY, 0.f);
+  if (t < a.splits) ml = reinterpret_cast<const float2*>(a.part_ml)[(long long)t * all_rows + row];
+  float top = ml.x;
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+  if (lane == 0) red[wave] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float w = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - top);     // 0: no key of the query there
+  weight[t] = w;
+  float l = w == 0.f ? 0.f : w * ml.y;
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) l += __shfl_xor(l, x);
+  if (lane == 0) red[4 + wave] = l;
+  __syncthreads();
+  l = (red[4] + red[5]) + (red[6] + red[7]);
+
+  const int ch = t % QP * 4;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (ch < a.d)
+    for (int z = t / QP; z < a.splits; z += G) {
+      const float4 o = *reinterpret_cast<const float4*>(a.part_o + ((long long)z * all_rows + row) * a.d + ch);
+      add_piece(v, weight[z], o);
+    }
+  sums[t] = v;
+  __syncthreads();
+  if (t >= QP || ch >= a.d) return;
+  for (int g = 1; g < G; ++g) {
+    const float4 o = sums[g * QP + t];
+    v = make_float4(v.x + o.x, v.y + o.y, v.z + o.z, v.w + o.w);
+  }
+  store_joined<T>(a, row, ch, v, l);
 }
 
 struct Shape {
   int waves, qtiles, splits;
 };
 
-// Queries of a workgroup: 32 per wave.  Where the query tiles do not fill the chip (256 compute units,
-// two workgroups of four waves or eight of one wave each) the key axis is cut into pieces of at least
-// 256 keys, joined by a second launch.
+// Queries of a workgroup: 32 per wave, four waves from 33 queries on.  Where the query tiles do not give
+// two workgroups per compute unit, the key axis is cut into pieces, joined by a second launch: of 64 keys at
+// least for single waves (one query, 8 heads, 2145 keys: 34 pieces 8.4, 9 pieces 9.7, 5 pieces 11.8 us), of 512
+// for four (300 queries and keys, 8 heads: whole 9.1, halves 10.5 us).  More workgroups than two per unit
+// cost more in joining than they hide (100 queries, 33153 keys, 2 x 8 heads: 512 of them 31, 2048 36 us).
 Shape shape_of(const fss_attention_desc& d) {
   Shape s;
   const long long rows = (long long)d.q_len * (d.q_heads / d.kv_heads);
   s.waves = rows > 32 ? 4 : 1;
   s.qtiles = ceil_div(rows, 32 * s.waves);
   const long long blocks = (long long)d.batch * d.kv_heads * s.qtiles;
-  const long long want = s.waves == 4 ? 512 : 2048;
-  long long splits = want / blocks, most = ceil_div(d.kv_len, 256);
+  long long splits = 512 / blocks, most = d.kv_len / (s.waves == 4 ? 512 : 64);
   if (splits > most) splits = most;
+  if (splits > kMaxSplits) splits = kMaxSplits;
   s.splits = splits > 1 ? (int)splits : 1;
   return s;
 }
@@ -443,11 +558,12 @@ size_t workspace_of(const fss_attention_desc& d, const Shape& s) {
 template <typename T, int DP, int NW>
 int launch(const AttnArgs& a, const Shape& s, hipStream_t stream) {
   const dim3 grid((unsigned)((long long)a.batch * a.kv_heads * a.qtiles * a.splits));
-  const size_t lds = 4 * Tile<DP>::kBytes;
+  const size_t lds = 2 * Tile<DP>::kBytes * (a.mask != nullptr ? kStages<DP, true> : kStages<DP, false>);
 #define FSS_ATTN(MASK, SPLIT)                                                                                       \
   do {                                                                                                              \
-    FSS_CHECK_HIP(hipFuncSetAttribute((const void*)attention_kernel<T, DP, NW, MASK, SPLIT>,                        \
-                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));                       \
+    if (lds > 64 * 1024)                                                                                            \
+      FSS_CHECK_HIP(hipFuncSetAttribute((const void*)attention_kernel<T, DP, NW, MASK, SPLIT>,                      \
+                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));                     \
     hipLaunchKernelGGL((attention_kernel<T, DP, NW, MASK, SPLIT>), grid, dim3(NW * 64), lds, stream, a);            \
   } while (0)
   if (a.mask != nullptr) {
@@ -521,11 +637,27 @@ int fss_cross_attention(const fss_attention_desc* desc, const void* q, const voi
   hipStream_t st = (hipStream_t)stream;
   const int e = d.dtype == FSS_F16 ? launch_type<f16_t>(a, s, st) : launch_type<bf16_t>(a, s, st);
   if (e != 0 || s.splits == 1) return e;
-  const long long threads = all_rows * (d.head_dim / 4);
-  FSS_REQUIRE((threads + 255) / 256 < 0x7fffffffLL, "too many rows");
-  const dim3 grid((unsigned)((threads + 255) / 256));
-  if (d.dtype == FSS_F16) hipLaunchKernelGGL(attention_join_kernel<f16_t>, grid, dim3(256), 0, st, a, all_rows);
-  else hipLaunchKernelGGL(attention_join_kernel<bf16_t>, grid, dim3(256), 0, st, a, all_rows);
+  if (s.splits <= kFewSplits) {
+    const long long threads = all_rows * (d.head_dim / 4);
+    const dim3 grid((unsigned)((threads + 255) / 256));
+    if (d.dtype == FSS_F16) hipLaunchKernelGGL(attention_join_few_kernel<f16_t>, grid, dim3(256), 0, st, a, all_rows);
+    else hipLaunchKernelGGL(attention_join_few_kernel<bf16_t>, grid, dim3(256), 0, st, a, all_rows);
+    FSS_LAUNCH_CHECK();
+    return 0;
+  }
+  const dim3 grid((unsigned)all_rows);
+#define FSS_JOIN(QP)                                                                                                 \
+  do {                                                                                                               \
+    if (d.dtype == FSS_F16)                                                                                          \
+      hipLaunchKernelGGL((attention_join_kernel<f16_t, QP>), grid, dim3(256), 0, st, a, (int)all_rows);              \
+    else                                                                                                             \
+      hipLaunchKernelGGL((attention_join_kernel<bf16_t, QP>), grid, dim3(256), 0, st, a, (int)all_rows);             \
+  } while (0)
+  if (d.head_dim <= 32) FSS_JOIN(8);
+  else if (d.head_dim <= 64) FSS_JOIN(16);
+  else if (d.head_dim <= 128) FSS_JOIN(32);
+  else FSS_JOIN(64);
+#undef FSS_JOIN
   FSS_LAUNCH_CHECK();
   return 0;
 }

@@ -431,8 +431,9 @@ int launch_tile(const MmArgs& a, hipStream_t stream) {
   const int tiles_n = ceil_div(a.cout, BN);
   const long long tiles = (a.rows + BM - 1) / BM * tiles_n;
   FSS_REQUIRE(tiles < 0x7fffffffLL, "too many tiles");
-  FSS_CHECK_HIP(hipFuncSetAttribute((const void*)matmul_fp8_tile_kernel<T, VEC, BM, BN, WM, WN, WK, NS>,
-                                    hipFuncAttributeMaxDynamicSharedMemorySize, L::kLds));
+  if (L::kLds > 64 * 1024)
+    FSS_CHECK_HIP(hipFuncSetAttribute((const void*)matmul_fp8_tile_kernel<T, VEC, BM, BN, WM, WN, WK, NS>,
+                                      hipFuncAttributeMaxDynamicSharedMemorySize, L::kLds));
   hipLaunchKernelGGL((matmul_fp8_tile_kernel<T, VEC, BM, BN, WM, WN, WK, NS>), dim3((unsigned)tiles), dim3(L::kThreads), L::kLds,
                      stream, a, tiles_n);
   FSS_LAUNCH_CHECK();
