@@ -6,9 +6,9 @@
 // e4m3 values from a zero accumulator, and its 4 results per lane are folded into the float sums
 // with one multiply-add each.  Operands are exchanged (D[channel][row] = w x^T), so that a lane's 4
 // results belong to ONE row of x and the block's factor sx * sw is one number per lane and MFMA.
-// The rows of a pair of weight tiles are interleaved (tile t takes channels 8 (r / 4) + 4 t + r % 4),
-// which leaves a lane with 8 consecutive channels of its row: 16-byte stores straight from the
-// accumulators.  The order of the 128 products inside an MFMA is free (both operands are read in the
+// The rows of a pair of weight tiles are interleaved (tile t takes channels 8 (r / 4) + 4 t + r % 4, put
+// side by side when they are copied to LDS), which leaves a lane with 8 consecutive channels of its row:
+// 16-byte stores straight from the accumulators.  The order of the 128 products inside an MFMA is free (both operands are read in the
 // same one), so a lane simply takes 16-byte pieces g and g + 4 of its row's 128 bytes.
 #include <type_traits>
 
@@ -293,7 +293,9 @@ matmul_fp8_tile_kernel(const MmArgs a, int tiles_n) {
 #pragma unroll
   for (int i = 0; i < L::kWPieces; ++i) {
     const int row = (wave * L::kWPieces + i) * 8 + prow, chunk = phys ^ ((row >> 1) & 7);
-    woff[i] = row < chans_left ? (unsigned)(row * (int)a.w_ld + chunk * 16) : kMmOutside + chunk * 16;
+    // rows of a fragment lie together: row 16 t + r of a pair holds channel 8 (r / 4) + 4 t + r % 4
+    const int chan = (row & ~31) + 8 * ((row & 15) >> 2) + (row >> 4 & 1) * 4 + (row & 3);
+    woff[i] = chan < chans_left ? (unsigned)(chan * (int)a.w_ld + chunk * 16) : kMmOutside + chunk * 16;
   }
   auto stage = [&](int kb, unsigned dst) {
     const unsigned k0 = (unsigned)kb * 128u;
@@ -328,12 +330,10 @@ matmul_fp8_tile_kernel(const MmArgs a, int tiles_n) {
     for (int i = 0; i < TI; ++i) acc[j][i] = fss_f32x4{0.f, 0.f, 0.f, 0.f};
 
   const int r = lane & 15, g = lane >> 4;
-  const int xswz = (r >> 1) & 7;
+  const int swz = (r >> 1) & 7;
   const char* px = ring + (wm * TJ * 16 + r) * 128;
   const char* psx = ring + L::kXBytes + L::kWBytes + (wm * TJ * 16 + r) * 4;
-  // weight rows of tile t of a pair: 8 (r / 4) + 4 t + r % 4
-  const int wrow0 = 8 * (r >> 2) + (r & 3), wswz0 = (wrow0 >> 1) & 7, wswz1 = ((wrow0 + 4) >> 1) & 7;
-  const char* pw = ring + L::kXBytes + (wn * TI * 16 + wrow0) * 128;
+  const char* pw = ring + L::kXBytes + (wn * TI * 16 + r) * 128;
   const char* psw = ring + L::kXBytes + L::kWBytes + BM * 4 + ((n0 & 127) + wn * TI * 16 >> 7) * 4;
   const bool more = wave <= BM / 64;           // this wave copies scales, too
 
@@ -362,8 +362,7 @@ matmul_fp8_tile_kernel(const MmArgs a, int tiles_n) {
     Block<T> fw[TI];
 #pragma unroll
     for (int i = 0; i < TI; ++i) {
-      const char* p = pw + cur + (i >> 1) * 32 * 128 + (i & 1) * 4 * 128;
-      const int swz = (i & 1) ? wswz1 : wswz0;
+      const char* p = pw + cur + i * 16 * 128;
       fw[i].set(*reinterpret_cast<const uint4*>(p + ((g ^ swz) << 4)),
                 *reinterpret_cast<const uint4*>(p + (((4 + g) ^ swz) << 4)));
     }
@@ -371,8 +370,8 @@ matmul_fp8_tile_kernel(const MmArgs a, int tiles_n) {
     for (int j = 0; j < TJ; ++j) {
       Block<T> fx;
       const char* p = px + cur + j * 16 * 128;
-      fx.set(*reinterpret_cast<const uint4*>(p + ((g ^ xswz) << 4)),
-             *reinterpret_cast<const uint4*>(p + (((4 + g) ^ xswz) << 4)));
+      fx.set(*reinterpret_cast<const uint4*>(p + ((g ^ swz) << 4)),
+             *reinterpret_cast<const uint4*>(p + (((4 + g) ^ swz) << 4)));
       const float s = sw * *reinterpret_cast<const float*>(psx + cur + j * 64);
 #pragma unroll
       for (int i = 0; i < TI; ++i) {
@@ -454,20 +453,20 @@ template <typename T>
 int launch_matmul(const MmArgs& a, hipStream_t stream) {
   auto tiles = [&](int bm, int bn) { return (a.rows + bm - 1) / bm * ceil_div(a.cout, bn); };
   // Rules measured over 1 to 132612 rows, 19 to 8192 channels and k from 128 to 8192 (us, 16-bit outputs):
-  //   few rows, while their work is at most 10 blocks of k per compute unit (1 x 512, k 2048: 5.0 against 7.6;
+  //   few rows, while their work is at most 10 blocks of k per compute unit (1 x 512, k 2048: 5.0 against 7.2;
   //   300 x 1024, k 1024: 8.0 against 6.1);
   if ((a.rows + 15) / 16 * ceil_div(a.cout, 32) * a.kblocks <= 2560) return launch_few<T>(a, stream);
 #define FSS_TILE(...) \
   return a.vec ? launch_tile<T, true, __VA_ARGS__>(a, stream) : launch_tile<T, false, __VA_ARGS__>(a, stream)
   //   256 x 256 where they fill whole rounds of the 256 compute units and k is long enough to hide a tile's
-  //   ends (8192 x 8192, k 8192: 528 against 590; 33153 x 1024, k 2048, 2.03 rounds: 112 against 97);
+  //   ends (8192 x 8192, k 8192: 504 against 578; 33153 x 1024, k 2048, 2.03 rounds: 110 against 94);
   const long long big = tiles(256, 256), rounds = (big + 255) / 256;
   if (big >= 240 && big * 10 >= rounds * 256 * 9 && a.kblocks >= 8) FSS_TILE(256, 256, 2, 4, 1, 2);
-  //   128 x 128 from three per compute unit (33153 x 1024, k 2048: 97 against 115; 8385 x 1024, k 1024,
+  //   128 x 128 from three per compute unit (33153 x 1024, k 2048: 94 against 129; 8385 x 1024, k 1024,
   //   528 tiles: 24.0 against 21.7);
   if (tiles(128, 128) >= 768) FSS_TILE(128, 128, 2, 2, 1, 2);
   //   64 x 64 with two groups of waves along k where the chain of its blocks is what takes the time (2145 x
-  //   512, k 2048: 10.7 against 11.6; 8385 x 256, k 1024: 11.4 against 9.3), else with one.
+  //   512, k 2048: 10.3 against 11.4; 8385 x 256, k 1024: 11.4 against 9.3), else with one.
   if (tiles(64, 64) <= 512 && a.kblocks >= 8) FSS_TILE(64, 64, 2, 2, 2, 2);
   FSS_TILE(64, 64, 2, 2, 1, 2);
 #undef FSS_TILE
