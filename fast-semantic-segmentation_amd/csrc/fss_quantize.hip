@@ -1,6 +1,6 @@
 // Storage conversion to 8-bit floating point with one float scale per block of 128 columns (gfx950):
 //
-//   a = max(largest |x| of the block, 2^-100),  s = a / 448,  q = e4m3(x * (448 / a))
+//   a = max(largest |x| of the block, 2^-100),  s = a / 448,  q = e4m3(448 x / a)
 //
 // for blocks of 1 row (activations) or 128 rows (weights).  HBM-bound: x is read once, q (one
 // byte) and the scales (4 bytes per 128 or 16384 elements) are written once; a block's values stay in
@@ -36,18 +36,46 @@ __device__ __forceinline__ unsigned amax16(const float (&v)[16]) {
   return a;
 }
 
-__device__ __forceinline__ void scale_of(unsigned amax_bits, float& scale, float& inv) {
-  const float a = __uint_as_float(max(amax_bits, kTinyBits));
+__device__ __forceinline__ void scale_of(unsigned amax_bits, float& a, float& scale, float& inv) {
+  a = __uint_as_float(max(amax_bits, kTinyBits));
   scale = amax_bits < kInfBits ? a / kE4m3Max : __uint_as_float(0x7fc00000u);
   inv = amax_bits < kInfBits ? kE4m3Max / a : __uint_as_float(0x7fc00000u);
 }
 
-__device__ __forceinline__ uint4 to_fp8(const float (&v)[16], float inv) {
+// The byte of one element whose quotient 448 x / a lies within 2^-20 of a midpoint: `hi` and `lo` are
+// the two e4m3 neighbours.  Compares 448 |x| with mid * a (both over 512: no overflow): values of T have at
+// most 16 bits (floats 24), so both products, and the side their difference is on, are exact.
+template <typename T> __device__ __forceinline__ unsigned settle(unsigned hi, unsigned lo, float x, float a) {
+  const float mid = 0x1p-10f * (fabsf(__builtin_amdgcn_cvt_f32_fp8((int)hi, 0)) + fabsf(__builtin_amdgcn_cvt_f32_fp8((int)lo, 0)));
+  float above;
+  if constexpr (__is_same(T, float)) above = (float)(0.875 * fabs((double)x) - (double)mid * (double)a);
+  else above = fmaf(-mid, a, 0.875f * fabsf(x));
+  return above > 0.f || (above == 0.f && (lo & 1)) ? hi : lo;
+}
+
+// In float, x * (448 / a) is within 2^-22 of the quotient.  Rounding it with 448 / a made larger and smaller by 2^-21
+// gives the same byte unless a midpoint lies between, and then it is the quotient's byte; where the two
+// differ (ties are common: bfloat16 values over a bfloat16 maximum), settle decides.
+template <typename T> __device__ __forceinline__ uint4 to_fp8(const float (&v)[16], float inv, float a) {
+  const float more = inv * (1.f + 0x1p-21f), less = inv * (1.f - 0x1p-21f);
   unsigned w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    int t = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i] * inv, v[4 * i + 1] * inv, 0, false);
-    w[i] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i + 2] * inv, v[4 * i + 3] * inv, t, true);
+    const float* x = v + 4 * i;
+    int hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * more, x[1] * more, 0, false);
+    int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * less, x[1] * less, 0, false);
+    hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[2] * more, x[3] * more, hi, true);
+    lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[2] * less, x[3] * less, lo, true);
+    w[i] = (unsigned)lo;
+    if (hi != lo) {
+      unsigned r = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const unsigned h = (unsigned)hi >> (8 * e) & 0xffu, l = (unsigned)lo >> (8 * e) & 0xffu;
+        r |= (h == l ? l : settle<T>(h, l, x[e], a)) << (8 * e);
+      }
+      w[i] = r;
+    }
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
@@ -72,9 +100,9 @@ quantize_rows_kernel(const T* __restrict__ x, long long x_ld, uint8_t* __restric
   unsigned a = amax16(v);
 #pragma unroll
   for (int d = 1; d < 8; d <<= 1) a = max(a, (unsigned)__shfl_xor((int)a, d));
-  float scale, inv;
-  scale_of(a, scale, inv);
-  if (in) *reinterpret_cast<uint4*>(q + row * q_ld + col) = to_fp8(v, inv);
+  float top, scale, inv;
+  scale_of(a, top, scale, inv);
+  if (in) *reinterpret_cast<uint4*>(q + row * q_ld + col) = to_fp8<T>(v, inv, top);
   if (part == 0 && row < rows) scales[kb * scale_ld + row] = scale;
 }
 
@@ -105,12 +133,12 @@ quantize_tiles_kernel(const T* __restrict__ x, long long x_ld, uint8_t* __restri
   if ((threadIdx.x & 63) == 0) wave_max[threadIdx.x >> 6] = a;
   __syncthreads();
   a = max(max(wave_max[0], wave_max[1]), max(wave_max[2], wave_max[3]));
-  float scale, inv;
-  scale_of(a, scale, inv);
+  float top, scale, inv;
+  scale_of(a, top, scale, inv);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const long long row = rb * 128 + i * 32 + (threadIdx.x >> 3);
-    if (row < rows && col < cols) *reinterpret_cast<uint4*>(q + row * q_ld + col) = to_fp8(v[i], inv);
+    if (row < rows && col < cols) *reinterpret_cast<uint4*>(q + row * q_ld + col) = to_fp8<T>(v[i], inv, top);
   }
   if (threadIdx.x == 0) scales[kb * scale_ld + rb] = scale;
 }

@@ -468,7 +468,7 @@ int fss_confusion_accumulate(const uint8_t* pred, const uint8_t* labels,
 /* q = x in 8-bit floating point (OCP e4m3: 4 exponent bits, 3 mantissa bits, largest 448) with a
  * float scale per block of `block_rows` (1 or 128) rows x 128 columns, x ~ q * scale:
  *   a = max(largest |x| of the block, 2^-100),  scale = a / 448,
- *   q = (x * (448 / a)) rounded to nearest even, in float.
+ *   q = the quotient 448 x / a, rounded once, to nearest even.
  * x: [rows][cols] of `dtype` (FSS_F32 | FSS_BF16 | FSS_F16 | FSS_F32_BF16X3), cols a multiple of 16,
  * row stride x_ld a multiple of 16 bytes (FSS_F32_BF16X3: of 32); q: row stride q_ld a multiple of 16;
  * scales: [ceil(cols/128)][ceil(rows/block_rows)], stride scale_ld between column blocks (rows

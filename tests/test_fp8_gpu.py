@@ -27,11 +27,11 @@ def test_quantize(rows, cols, block_rows, x_pad, q_pad, scale_pad, dt):
     # scale: one division, half a step of float
     np.testing.assert_allclose(scales, ref_scales, rtol=2.0 ** -24, atol=0)
     # values: within half an e4m3 step of x / scale (2^-4 relative, 2^-10 below the smallest normal
-    # 2^-6), widened by the float product and quotient in front of the rounding (2 * 2^-24)
+    # 2^-6), widened by the rounding of the scale (2^-24)
     spread = U.spread(ref_scales, block_rows, rows, cols)
     want = value.astype(np.float64) / spread
     assert np.all(np.abs(q - want) <= np.maximum(np.abs(want) * (2.0 ** -4 + 2.0 ** -22), 2.0 ** -10 * (1 + 2.0 ** -20)))
-    # and equal to the float formula, bit for bit
+    # and equal to the exact quotient's rounding, ties included
     assert np.array_equal(q, ref_q)
     assert np.all(raw[:, cols:] == 0x55) and raw.shape[1] == cols + q_pad
 
@@ -54,6 +54,24 @@ def test_quantize_extremes(block_rows):
     np.testing.assert_array_equal(np.isnan(scales), np.isnan(ref_scales))
     np.testing.assert_array_equal(q, ref_q)
     assert np.isnan(scales).any() and not np.isnan(scales[0, -1])
+
+
+@gpu
+@pytest.mark.parametrize('dt', ['bf16', 'f16', 'f32'])
+@pytest.mark.parametrize('top', [448.0, 7.0, 3.5, 1.3125, 0.013671875, 57344.0, 2.0 ** 127, 2.0 ** -90])
+def test_quantize_ties(dt, top):
+    """Quotients on and next to the midpoints of e4m3, in its normal and subnormal range."""
+    k = np.arange(256, dtype=np.float64)
+    mids = np.concatenate([(16 + k[:16] + 0.5) / 16 * 2.0 ** e for e in range(-6, 9)] + [(k[:16] + 0.5) * 2.0 ** -9])
+    x = np.concatenate([mids * s * top / 448 for s in (1, -1, 1 + 2.0 ** -23, 1 - 2.0 ** -23, 1 + 2.0 ** -8)])
+    x = np.resize(x[np.abs(x) <= top], (31, 128)).astype(np.float32)
+    x[:, 5] = top
+    if dt == 'f16' and not 2.0 ** -8 <= top <= 65504:
+        return
+    stored, value = U.store(x, dt, 128)
+    for block_rows in (1, 128):
+        q, _, _ = U.quantize(stored, 31, 128, block_rows, dt)
+        assert np.array_equal(q, U.quantize_ref(value, block_rows)[0])
 
 
 # --------------------------------------------------------------------------------------- matmul
