@@ -10,6 +10,7 @@
 // side by side when they are copied to LDS), which leaves a lane with 8 consecutive channels of its row:
 // 16-byte stores straight from the accumulators.  The order of the 128 products inside an MFMA is free (both operands are read in the
 // same one), so a lane simply takes 16-byte pieces g and g + 4 of its row's 128 bytes.
+#include <algorithm>
 #include <type_traits>
 
 #include "fss_conv_args.h"
@@ -28,7 +29,9 @@ struct MmArgs {
   const void* res;
   void* y;
   long long rows, x_ld, x_scale_ld, w_ld, w_scale_ld, res_ld, y_ld;
-  int cout, k, kblocks, act, vec;   // vec: y, residual and their strides allow 16-byte accesses
+  int cout, k, kblocks, act, vec;   // vec: cout, y, residual and their strides allow 16-byte accesses
+  float* part;                      // k split over the grid: [splits][rows][part_ld] sums, else null
+  int splits, per, part_ld;         // blocks of k per split
 };
 
 // 16 e4m3 values of a lane as two operands of 8 half-precision values (exact)
@@ -258,7 +261,7 @@ __device__ __forceinline__ void blds4(unsigned voff, fss_i32x4 rsrc, unsigned ld
       : "memory", "m0");
 }
 
-template <typename T, bool VEC, int BM, int BN, int WM, int WN, int WK, int NS>
+template <typename T, bool VEC, bool PART, int BM, int BN, int WM, int WN, int WK, int NS>
 __global__ void __launch_bounds__(64 * WM * WN * WK, 2)
 matmul_fp8_tile_kernel(const MmArgs a, int tiles_n) {
   typedef MmTile<BM, BN, WM, WN, WK, NS> L;
@@ -275,6 +278,8 @@ matmul_fp8_tile_kernel(const MmArgs a, int tiles_n) {
   const int nwg = gridDim.x, bid = blockIdx.x;
   const int q8 = nwg >> 3, rr = nwg & 7, xcd = bid & 7;
   const int wg = (xcd < rr ? xcd * (q8 + 1) : rr * (q8 + 1) + (xcd - rr) * q8) + (bid >> 3);
+  const int kb0 = PART ? blockIdx.y * a.per : 0, kcount = PART ? min(a.per, a.kblocks - kb0) : a.kblocks;
+  const int kend = PART ? min(a.k, (kb0 + kcount) * 128) : a.k;
   const int tiles_m = nwg / tiles_n, band = wg / (8 * tiles_n), in_band = wg - band * 8 * tiles_n;
   const int band_m = min(8, tiles_m - band * 8);
   const long long m0 = (long long)(band * 8 + in_band % band_m) * BM;
@@ -299,17 +304,17 @@ matmul_fp8_tile_kernel(const MmArgs a, int tiles_n) {
   }
   auto stage = [&](int kb, unsigned dst) {
     const unsigned k0 = (unsigned)kb * 128u;
-    const bool whole = (int)k0 + 128 <= a.k, past = kb >= a.kblocks;            // uniform
+    const bool whole = (int)k0 + 128 <= kend, past = (int)k0 >= kend;            // uniform
 #pragma unroll
     for (int i = 0; i < L::kXPieces; ++i) {
       const int row = (wave * L::kXPieces + i) * 8 + prow, chunk = phys ^ ((row >> 1) & 7);
-      blds16(whole || (int)k0 + chunk * 16 < a.k ? xoff[i] + k0 : kMmOutside, rx,
+      blds16(whole || (int)k0 + chunk * 16 < kend ? xoff[i] + k0 : kMmOutside, rx,
              dst + (wave * L::kXPieces + i) * 1024);
     }
 #pragma unroll
     for (int i = 0; i < L::kWPieces; ++i) {
       const int row = (wave * L::kWPieces + i) * 8 + prow, chunk = phys ^ ((row >> 1) & 7);
-      blds16(whole || (int)k0 + chunk * 16 < a.k ? woff[i] + k0 : kMmOutside, rw,
+      blds16(whole || (int)k0 + chunk * 16 < kend ? woff[i] + k0 : kMmOutside, rw,
              dst + L::kXBytes + (wave * L::kWPieces + i) * 1024);
     }
     const unsigned sdst = dst + L::kXBytes + L::kWBytes + wave * 256;
@@ -339,10 +344,10 @@ matmul_fp8_tile_kernel(const MmArgs a, int tiles_n) {
 
   // blocks wk, wk + WK, ... of k; all groups make the same number of rounds (a round past the end of
   // k deposits zeros), as they share the barriers
-  const int rounds = (a.kblocks + WK - 1) / WK;
+  const int rounds = (kcount + WK - 1) / WK;
 #pragma unroll
   for (int i = 0; i < NS - 1; ++i)
-    if (i < rounds) stage(i * WK + wk, ring_base + i * L::kStage);
+    if (i < rounds) stage(kb0 + i * WK + wk, ring_base + i * L::kStage);
   unsigned cur = 0, ahead = (NS - 1) * L::kStage;
   for (int round = 0; round < rounds; ++round) {
     // everything but the stages behind this one (those that exist) has landed
@@ -357,7 +362,7 @@ matmul_fp8_tile_kernel(const MmArgs a, int tiles_n) {
       wait_vmcnt<0>();
     }
     __syncthreads();       // ... for every wave, and nobody reads the stage refilled next any more
-    if (round + NS - 1 < rounds) stage((round + NS - 1) * WK + wk, ring_base + ahead);
+    if (round + NS - 1 < rounds) stage(kb0 + (round + NS - 1) * WK + wk, ring_base + ahead);
     const float sw = *reinterpret_cast<const float*>(psw + cur);
     Block<T> fw[TI];
 #pragma unroll
@@ -419,9 +424,48 @@ matmul_fp8_tile_kernel(const MmArgs a, int tiles_n) {
         v[e] = acc[j][i][e];
         v[4 + e] = acc[j][i + 1][e];
       }
-      if (row < rows_left) finish8<T, VEC>(a, lim, m0 + row, n0 + c0, v);
+      if (row >= rows_left) continue;
+      if constexpr (PART) store8(a.part + ((long long)blockIdx.y * a.rows + m0 + row) * a.part_ld + n0 + c0, v);
+      else finish8<T, VEC>(a, lim, m0 + row, n0 + c0, v);
     }
   }
+}
+
+// Adds the splits in index order and finishes 8 channels of a row per thread.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) matmul_fp8_join_kernel(const MmArgs a) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int units = a.part_ld / 8;
+  const long long row = i / units;
+  if (row >= a.rows) return;
+  const int c0 = (int)(i - row * units) * 8;
+  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int z = 0; z < a.splits; ++z) {
+    float t[8];
+    load8(a.part + (z * a.rows + row) * a.part_ld + c0, t);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += t[e];
+  }
+  finish8<T, VEC>(a, limits_of<T>(a.act), row, c0, v);
+}
+
+// 64 x 64 tiles with k split over the grid
+template <typename T>
+int launch_split(const MmArgs& a, hipStream_t stream) {
+  typedef MmTile<64, 64, 2, 2, 2, 2> L;
+  typedef std::conditional_t<sizeof(T) == 4, float, bf16_t> M;            // which products, nothing else
+  const auto kern = matmul_fp8_tile_kernel<M, true, true, 64, 64, 2, 2, 2, 2>;
+  FSS_CHECK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, L::kLds));
+  const int tiles_n = ceil_div(a.cout, 64);
+  const dim3 grid((unsigned)((a.rows + 63) / 64 * tiles_n), a.splits);
+  hipLaunchKernelGGL(kern, grid, dim3(L::kThreads), L::kLds, stream, a, tiles_n);
+  FSS_LAUNCH_CHECK();
+  const dim3 join((unsigned)((a.rows * (a.part_ld / 8) + 255) / 256));
+  if (a.vec) hipLaunchKernelGGL((matmul_fp8_join_kernel<T, true>), join, dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((matmul_fp8_join_kernel<T, false>), join, dim3(256), 0, stream, a);
+  FSS_LAUNCH_CHECK();
+  return 0;
 }
 
 template <typename T, bool VEC, int BM, int BN, int WM, int WN, int WK, int NS>
@@ -431,9 +475,9 @@ int launch_tile(const MmArgs& a, hipStream_t stream) {
   const long long tiles = (a.rows + BM - 1) / BM * tiles_n;
   FSS_REQUIRE(tiles < 0x7fffffffLL, "too many tiles");
   if (L::kLds > 64 * 1024)
-    FSS_CHECK_HIP(hipFuncSetAttribute((const void*)matmul_fp8_tile_kernel<T, VEC, BM, BN, WM, WN, WK, NS>,
+    FSS_CHECK_HIP(hipFuncSetAttribute((const void*)matmul_fp8_tile_kernel<T, VEC, false, BM, BN, WM, WN, WK, NS>,
                                       hipFuncAttributeMaxDynamicSharedMemorySize, L::kLds));
-  hipLaunchKernelGGL((matmul_fp8_tile_kernel<T, VEC, BM, BN, WM, WN, WK, NS>), dim3((unsigned)tiles), dim3(L::kThreads), L::kLds,
+  hipLaunchKernelGGL((matmul_fp8_tile_kernel<T, VEC, false, BM, BN, WM, WN, WK, NS>), dim3((unsigned)tiles), dim3(L::kThreads), L::kLds,
                      stream, a, tiles_n);
   FSS_LAUNCH_CHECK();
   return 0;
@@ -449,13 +493,27 @@ int launch_few(const MmArgs& a, hipStream_t stream) {
   return 0;
 }
 
+// Rules measured over 1 to 132612 rows, 19 to 8192 channels and k from 128 to 16384 (us, 16-bit outputs).
+// Few rows, while their work is at most 10 blocks of k per compute unit (1 x 512, k 2048: 5.0 against 7.2;
+// 300 x 1024, k 1024: 8.0 against 6.1).
+bool few_rows(long long rows, int cout, int kblocks) {
+  return (rows + 15) / 16 * ceil_div(cout, 32) * kblocks <= 2560;
+}
+// Pieces of k for the grid, where few 64 x 64 tiles meet a long k: to one workgroup per compute unit, of 8
+// blocks each at least (128 x 128, k 16384: 16 pieces 9.4 against 33.0 us whole; 512 x 512, k 8192: 4 pieces 14.3
+// against 24.4; 300 x 1024, k 2048, 80 tiles: 2 pieces 9.2 against 7.8).
+int splits_of(long long rows, int cout, int kblocks) {
+  const long long tiles = (rows + 63) / 64 * ceil_div(cout, 64);
+  if (few_rows(rows, cout, kblocks) || tiles > 64 || kblocks < 32) return 1;
+  const long long splits = std::min(256 / tiles, (long long)kblocks / 8);
+  return (int)std::min(splits, 16ll);
+}
+
 template <typename T>
 int launch_matmul(const MmArgs& a, hipStream_t stream) {
   auto tiles = [&](int bm, int bn) { return (a.rows + bm - 1) / bm * ceil_div(a.cout, bn); };
-  // Rules measured over 1 to 132612 rows, 19 to 8192 channels and k from 128 to 8192 (us, 16-bit outputs):
-  //   few rows, while their work is at most 10 blocks of k per compute unit (1 x 512, k 2048: 5.0 against 7.2;
-  //   300 x 1024, k 1024: 8.0 against 6.1);
-  if ((a.rows + 15) / 16 * ceil_div(a.cout, 32) * a.kblocks <= 2560) return launch_few<T>(a, stream);
+  if (few_rows(a.rows, a.cout, a.kblocks)) return launch_few<T>(a, stream);
+  if (a.splits > 1) return launch_split<T>(a, stream);
 #define FSS_TILE(...) \
   return a.vec ? launch_tile<T, true, __VA_ARGS__>(a, stream) : launch_tile<T, false, __VA_ARGS__>(a, stream)
   //   256 x 256 where they fill whole rounds of the 256 compute units and k is long enough to hide a tile's
@@ -470,6 +528,11 @@ int launch_matmul(const MmArgs& a, hipStream_t stream) {
   if (tiles(64, 64) <= 512 && a.kblocks >= 8) FSS_TILE(64, 64, 2, 2, 2, 2);
   FSS_TILE(64, 64, 2, 2, 1, 2);
 #undef FSS_TILE
+}
+
+size_t workspace_of(const fss_matmul_fp8_desc& d) {
+  const int splits = splits_of(d.rows, d.cout, ceil_div(d.k, 128));
+  return splits == 1 ? 0 : (size_t)splits * d.rows * ceil_div(d.cout, 8) * 8 * sizeof(float);
 }
 
 int check_desc(const fss_matmul_fp8_desc* d) {
@@ -492,7 +555,7 @@ extern "C" {
 int fss_matmul_fp8_workspace_bytes(const fss_matmul_fp8_desc* desc, size_t* bytes) {
   FSS_REQUIRE(bytes != nullptr, "null argument");
   if (int e = check_desc(desc)) return e;
-  *bytes = 0;
+  *bytes = workspace_of(*desc);
   return 0;
 }
 
@@ -525,6 +588,14 @@ int fss_matmul_fp8(const fss_matmul_fp8_desc* desc, const void* x, const float* 
   a.cout = d.cout; a.k = d.k; a.kblocks = ceil_div(d.k, 128); a.act = d.act;
   a.vec = d.cout % 8 == 0 && (((uintptr_t)y | (uintptr_t)residual) & 15) == 0 && d.y_ld * es % 16 == 0 &&
           (residual == nullptr || d.res_ld * es % 16 == 0);
+  const size_t need = workspace_of(d);
+  FSS_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
+              "workspace missing, too small or unaligned");
+  a.splits = splits_of(d.rows, d.cout, a.kblocks);
+  a.per = ceil_div(a.kblocks, a.splits);
+  a.splits = ceil_div(a.kblocks, a.per);
+  a.part = (float*)workspace;
+  a.part_ld = ceil_div(d.cout, 8) * 8;
   hipStream_t s = (hipStream_t)stream;
   if (d.out_dtype == FSS_F32) return launch_matmul<float>(a, s);
   if (d.out_dtype == FSS_BF16) return launch_matmul<bf16_t>(a, s);

@@ -79,7 +79,11 @@ MATMUL = [
     # rows, cout, k
     (1, 1, 16), (1, 512, 2048), (2, 19, 144), (7, 33, 128), (16, 64, 4096), (17, 129, 272), (33, 256, 512),
     (64, 64, 128), (100, 256, 256), (128, 128, 384), (129, 260, 1040), (255, 513, 528), (300, 72, 8192),
-    (1000, 19, 512), (2145, 512, 64), (4097, 136, 160), (8385, 300, 272)]
+    (1000, 19, 512), (2145, 512, 64), (4097, 136, 160), (8385, 300, 272),
+    # k split over the grid
+    (128, 128, 16384), (500, 130, 4240), (700, 19, 4224),
+    # the larger tiles
+    (16500, 520, 144), (8100, 2049, 1040), (4093, 4090, 1040)]
 
 
 @gpu
@@ -92,7 +96,7 @@ def test_matmul(rows, cout, k, dt, act, bias, residual):
 
 
 @gpu
-@pytest.mark.parametrize('rows,cout,k', [(1, 8, 16), (50, 136, 272), (1500, 264, 512)])
+@pytest.mark.parametrize('rows,cout,k', [(1, 8, 16), (50, 136, 272), (1500, 264, 512), (300, 72, 8192)])
 def test_matmul_split_bf16_output(rows, cout, k):
     U.check_matmul(rows, cout, k, 'f32x3', 'relu', True, True, y_pad=8)
 
@@ -168,6 +172,11 @@ def test_matmul_refusals():
                                       y_ld=24, res_ld=24), **bad))
         _refused('fss_matmul_fp8', ctypes.byref(d), *[1 << 12] * 7, None, 0, None)
     size = ctypes.c_size_t()
+    d = U.matmul_desc(300, 256, 8192, 'f32')
+    _lib.call('fss_matmul_fp8_workspace_bytes', ctypes.byref(d), ctypes.byref(size))
+    assert size.value > 0
+    for ws, n in ((None, size.value), (1 << 12, size.value - 1), ((1 << 12) + 8, size.value), (None, 0)):
+        _refused('fss_matmul_fp8', ctypes.byref(d), *[1 << 12] * 4, None, None, 1 << 12, ws, n, None)
     _refused('fss_matmul_fp8_workspace_bytes', ctypes.byref(U.matmul_desc(8, 24, 100, 'f32')), ctypes.byref(size))
     _refused('fss_matmul_fp8_workspace_bytes', ctypes.byref(U.matmul_desc(8, 24, 128, 'f32')), None)
     _refused('fss_matmul_fp8_workspace_bytes', None, ctypes.byref(size))
