@@ -11,6 +11,8 @@
 // one factor per lane, and the rounded p are the second product's operand where they are: its 16 keys may
 // be taken in any order as long as V is read in the same one, which the transposing LDS read
 // (ds_read_b64_tr_b16: 4 keys x 16 channels -> 4 keys per lane) does at no cost.
+#include <algorithm>
+
 #include "fss_conv_args.h"
 
 namespace fss {
@@ -401,27 +403,42 @@ attention_kernel(const AttnArgs a) {
       (void)sum;
     }
   }
-  if (!row_ok) return;
   if constexpr (SPLIT) {
-    if (h == 0) {
+    if (row_ok && h == 0) {
       a.part_ml[part * 2] = m;
       a.part_ml[part * 2 + 1] = l;
     }
   }
-  if (done) return;
+  if constexpr (SPLIT) {
+    if (done || !row_ok) return;
 #pragma unroll
-  for (int dt = 0; dt < DP / 32; ++dt)
+    for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int ch = dt * 32 + 8 * j + 4 * h;
-      if (ch >= a.d) continue;
-      const float v0 = o[dt][4 * j], v1 = o[dt][4 * j + 1], v2 = o[dt][4 * j + 2], v3 = o[dt][4 * j + 3];
-      if constexpr (SPLIT)
-        *reinterpret_cast<float4*>(a.part_o + part * a.d + ch) = make_float4(v0, v1, v2, v3);
-      else
-        *reinterpret_cast<uint2*>(yp + ch * 2) =
-            l == 0.f ? make_uint2(0, 0) : make_uint2(pack2_sat<T>(v0 * f, v1 * f), pack2_sat<T>(v2 * f, v3 * f));
-    }
+      for (int j = 0; j < 4; ++j) {
+        const int ch = dt * 32 + 8 * j + 4 * h;
+        if (ch < a.d)
+          *reinterpret_cast<float4*>(a.part_o + part * a.d + ch) =
+              make_float4(o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]);
+      }
+  } else {
+    // lanes l and l + 32 hold 4 channels each of 8; an exchange of two such groups leaves each lane with 8
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+      for (int j = 0; j < 4; j += 2) {
+        unsigned w[2][2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          w[0][e] = l == 0.f ? 0u : pack2_sat<T>(o[dt][4 * j + 2 * e] * f, o[dt][4 * j + 2 * e + 1] * f);
+          w[1][e] = l == 0.f ? 0u : pack2_sat<T>(o[dt][4 * j + 4 + 2 * e] * f, o[dt][4 * j + 5 + 2 * e] * f);
+        }
+        const auto t0 = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
+        const auto t1 = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
+        const int ch = dt * 32 + 8 * (j + h);
+        if (row_ok && !done && ch < a.d)
+          *reinterpret_cast<uint4*>(yp + ch * 2) = make_uint4(t0[0], t1[0], t0[1], t1[1]);
+      }
+  }
 }
 
 // y of a row's 4 channels from their joined sums
@@ -558,7 +575,9 @@ size_t workspace_of(const fss_attention_desc& d, const Shape& s) {
 template <typename T, int DP, int NW>
 int launch(const AttnArgs& a, const Shape& s, hipStream_t stream) {
   const dim3 grid((unsigned)((long long)a.batch * a.kv_heads * a.qtiles * a.splits));
-  const size_t lds = 2 * Tile<DP>::kBytes * (a.mask != nullptr ? kStages<DP, true> : kStages<DP, false>);
+  // a piece of the key axis with fewer tiles than buffers touches no more buffers than it has tiles
+  const int tiles = std::max(1, ceil_div(ceil_div(a.kv_len, kKeys), a.splits));
+  const size_t lds = 2 * Tile<DP>::kBytes * std::min(tiles, a.mask != nullptr ? kStages<DP, true> : kStages<DP, false>);
 #define FSS_ATTN(MASK, SPLIT)                                                                                       \
   do {                                                                                                              \
     if (lds > 64 * 1024)                                                                                            \
