@@ -108,7 +108,7 @@ __device__ __forceinline__ void blds16_at(unsigned voff, fss_i32x4 rsrc, unsigne
 }
 
 template <typename T, int DP, int NW, bool MASK, bool SPLIT>
-__global__ void __launch_bounds__(NW * 64, DP <= 64 ? 3 : DP <= 128 ? 2 : 1)
+__global__ void __launch_bounds__(NW * 64, DP <= 64 ? 3 : DP <= 128 || NW == 8 ? 2 : 1)
 attention_kernel(const AttnArgs a) {
   typedef Tile<DP> L;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
@@ -585,8 +585,10 @@ int launch(const AttnArgs& a, const Shape& s, hipStream_t stream) {
                                         hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));                     \
     hipLaunchKernelGGL((attention_kernel<T, DP, NW, MASK, SPLIT>), grid, dim3(NW * 64), lds, stream, a);            \
   } while (0)
-  if (a.mask != nullptr) {
-    if (s.splits > 1) FSS_ATTN(true, true); else FSS_ATTN(true, false);
+  if (NW < 8 && a.mask != nullptr) {
+    if constexpr (NW < 8) {
+      if (s.splits > 1) FSS_ATTN(true, true); else FSS_ATTN(true, false);
+    }
   } else {
     if (s.splits > 1) FSS_ATTN(false, true); else FSS_ATTN(false, false);
   }
@@ -601,6 +603,7 @@ int launch_type(const AttnArgs& a, const Shape& s, hipStream_t stream) {
   if (a.d <= 32) FSS_DP(32);
   if (a.d <= 64) FSS_DP(64);
   if (a.d <= 128) FSS_DP(128);
+  if (s.waves == 8) return launch<T, 256, 8>(a, s, stream);
   FSS_DP(256);
 #undef FSS_DP
 }
@@ -635,9 +638,17 @@ int fss_cross_attention(const fss_attention_desc* desc, const void* q, const voi
   }
   FSS_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)y | (uintptr_t)workspace) & 15) == 0 &&
                   ((uintptr_t)kv_lens & 3) == 0, "unaligned pointer");
-  const Shape s = shape_of(d);
+  Shape s = shape_of(d);
   const size_t need = workspace_of(d, s);
   FSS_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), "workspace too small");
+  // Eight waves with head_dim above 128, where the tiles leave LDS for one workgroup per compute unit (8 heads,
+  // 4096 queries and keys, head_dim 256: 195 against 260 us); not with a mask, whose registers would
+  // not fit (416 against 259 us).
+  const long long rows = (long long)d.q_len * (d.q_heads / d.kv_heads);
+  if (d.head_dim > 128 && rows > 128 && mask == nullptr) {
+    s.waves = 8;
+    s.qtiles = ceil_div(rows, 256);
+  }
   AttnArgs a;
   a.q = (const char*)q; a.k = (const char*)k; a.v = (const char*)v; a.y = (char*)y;
   a.lens = kv_lens; a.mask = mask;
