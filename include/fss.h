@@ -497,12 +497,14 @@ int fss_matmul_fp8_workspace_bytes(const fss_matmul_fp8_desc* desc, size_t* byte
 
 /* y = act( sum_b x_scale[b][m] * w_scale[b][n / 128] * (x[m][b] . w[n][b]) + bias[n] [+ residual[m][n]] )
  * over the blocks b of 128 along k: the product of two tensors fss_quantize_fp8 made, x with
- * block_rows 1 and w with block_rows 128, with fss_conv2d_nhwc's epilogue.  The products of a block are
- * summed on the matrix cores, blocks are scaled and summed in float, the result is rounded once, to
- * out_dtype (FSS_F16 saturates).  With 16-bit outputs the 8-bit matrix instructions are used, which drop
- * what lies below 2^-13 of the largest of 8 products (2e-5 of the result's size); with FSS_F32 and
- * FSS_F32_BF16X3 the same values go through the half-precision ones, which sum to float accuracy.  x, w, bias and workspace: 16-byte aligned, y and
- * residual aligned to their element (FSS_F32_BF16X3: 32 bytes).  bias, residual: NULL = none. */
+ * block_rows 1 and w with block_rows 128, with fss_conv2d_nhwc's epilogue.  The products of a block
+ * are summed on the matrix cores, blocks are scaled and summed in float, the result is rounded once,
+ * to out_dtype (FSS_F16 saturates).  With 16-bit outputs the 8-bit matrix instructions are used,
+ * which drop what lies below 2^-13 of the largest of 8 products (2e-5 of the result's size); with
+ * FSS_F32 and FSS_F32_BF16X3 the same values go through the half-precision ones, which sum to float
+ * accuracy.  x, w, bias and workspace: 16-byte aligned, y and residual aligned to their element
+ * (FSS_F32_BF16X3: 32 bytes), x_ld and w_ld multiples of 16 below 2^23.  bias, residual: NULL =
+ * none.  Rows and channels of any number; every sum is taken in a fixed order. */
 int fss_matmul_fp8(const fss_matmul_fp8_desc* desc, const void* x, const float* x_scales,
                    const void* w, const float* w_scales, const float* bias, const void* residual,
                    void* y, void* workspace, size_t workspace_bytes, void* stream);
@@ -529,10 +531,10 @@ int fss_cross_attention_workspace_bytes(const fss_attention_desc* desc, size_t* 
  * over the keys j < kv_lens[b] (NULL: kv_len; values are clamped to 0 .. kv_len) whose
  * mask[b,i,h,j] is not 0 (uint8, consecutive along j; NULL: all).  A query without any such key
  * gets zeros.  Keys and values at or behind kv_lens[b] are not read; a masked key has no effect
- * whatever its key and value hold, infinities and NaN included.  Scores, maximum, sums and
- * the output are accumulated in float; p is rounded to `dtype` for the product with v, y once at the
- * end (FSS_F16 saturates).  q, k, v, y, workspace: 16-byte aligned.  kv_lens is read on the device, so a captured
- * call follows its later contents. */
+ * whatever its key and value hold, infinities and NaN included.  Scores, maximum, sums and the
+ * output are accumulated in float; p is rounded to `dtype` (for the product with v and for the sum
+ * alike), y once at the end (FSS_F16 saturates).  q, k, v, y and workspace: 16-byte aligned.
+ * kv_lens is read on the device, so a captured call follows its later contents. */
 int fss_cross_attention(const fss_attention_desc* desc, const void* q, const void* k, const void* v,
                         const int32_t* kv_lens, const uint8_t* mask, void* y, void* workspace,
                         size_t workspace_bytes, void* stream);

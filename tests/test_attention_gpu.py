@@ -27,7 +27,8 @@ SHAPES = [
     (1, 1, 1, 1, 1, 8), (1, 1, 2145, 8, 8, 32), (2, 1, 700, 8, 2, 64), (1, 3, 63, 2, 1, 128), (2, 5, 64, 6, 2, 40),
     (1, 32, 65, 1, 1, 256), (1, 33, 129, 2, 2, 72), (3, 100, 1000, 4, 4, 32), (1, 128, 127, 3, 3, 96),
     (1, 130, 50, 8, 8, 64), (2, 257, 191, 4, 1, 128), (1, 600, 320, 7, 1, 16), (1, 70, 515, 2, 1, 200), (1, 129, 1, 2, 2, 64),
-    (1, 2000, 50, 8, 8, 64), (1, 31, 4000, 1, 1, 256), (4, 1, 33, 14, 2, 136)]
+    (1, 2000, 50, 8, 8, 64), (1, 31, 4000, 1, 1, 256), (4, 1, 33, 14, 2, 136),
+    (1, 200, 2600, 2, 1, 256), (1, 64, 1500, 4, 4, 160), (2, 90, 1100, 3, 3, 24), (1, 150, 1200, 2, 2, 64)]
 
 
 @gpu

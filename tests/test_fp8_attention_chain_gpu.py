@@ -175,6 +175,51 @@ def test_two_decoders_at_once():
         _lib.call('fss_graph_destroy', g)
 
 
+def test_first_call_under_capture():
+    """No warm-up call on these sizes: the largest tiles and the widest heads, which ask for more than 64 KiB of LDS."""
+    g = torch.Generator(device='cuda').manual_seed(4)
+    q, k, v = (torch.randn(1, n, 2, 248, generator=g, device='cuda').to(torch.float16) for n in (300, 700, 700))
+    y = torch.zeros_like(q)
+    ad = U.attention_desc(1, 300, 700, 2, 2, 248, 'f16')
+    rows, cout, k8 = 4096, 4096, 1024
+    x8 = torch.randint(0, 120, (rows, k8), generator=g, device='cuda', dtype=torch.uint8)
+    w8 = torch.randint(0, 120, (cout, k8), generator=g, device='cuda', dtype=torch.uint8)
+    xs, ws = torch.full((8, rows), 1e-3, device='cuda'), torch.full((8, 32), 1e-3, device='cuda')
+    out = torch.zeros(rows, cout, dtype=torch.float16, device='cuda')
+    md = U.matmul_desc(rows, cout, k8, 'f16')
+    size = ctypes.c_size_t()
+    _lib.call('fss_cross_attention_workspace_bytes', ctypes.byref(ad), ctypes.byref(size))
+    buf = torch.empty(size.value + 16, dtype=torch.uint8, device='cuda')
+    torch.cuda.synchronize()
+
+    def run():
+        _lib.call('fss_matmul_fp8', ctypes.byref(md), x8.data_ptr(), xs.data_ptr(), w8.data_ptr(), ws.data_ptr(), None, None,
+                  out.data_ptr(), None, 0, U.stream())
+        _lib.call('fss_cross_attention', ctypes.byref(ad), q.data_ptr(), k.data_ptr(), v.data_ptr(), None, None, y.data_ptr(),
+                  buf.data_ptr(), size.value, U.stream())
+
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        _lib.call('fss_capture_begin', U.stream())
+        run()
+        graph = ctypes.c_void_p()
+        _lib.call('fss_capture_end', U.stream(), ctypes.byref(graph))
+        got = []
+        for _ in range(3):
+            y.zero_()
+            out.zero_()
+            _lib.call('fss_graph_launch', graph, U.stream())
+            s.synchronize()
+            got.append((y.clone(), out.clone()))
+        run()
+        s.synchronize()
+    torch.cuda.synchronize()
+    for a, b in got:
+        assert torch.equal(a, y) and torch.equal(b, out) and out.abs().max() > 0
+    U.check_attention(y, U.attention_ref(q, k, v), 'f16', 248, 700)
+    _lib.call('fss_graph_destroy', graph)
+
+
 def test_matmul_and_quantize_past_4_gib():
     """Row offsets past 2^32 bytes: the last rows equal those of a small call on the same rows."""
     rows, k, cout = (1 << 20) + 70, 4096 + 128, 24
