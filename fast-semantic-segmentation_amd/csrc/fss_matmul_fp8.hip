@@ -127,38 +127,44 @@ template <typename T> __device__ __forceinline__ void store1(T* p, float v) {
   else ElemTraits<T>::store(p, v);
 }
 
-// Bias, residual, activation and store of 8 consecutive channels of one row that exists.  VEC: cout and
-// the strides allow 16-byte accesses.  (Two kernels instead of a branch: a launch that does little
-// is bound by fetching its instructions.)
+// Bias and residual of 8 consecutive channels of a row, as far as they exist
+template <typename T, bool VEC>
+__device__ __forceinline__ void bias8(const MmArgs& a, int c0, float (&v)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = 0.f;
+  if (a.bias == nullptr) return;
+  if constexpr (VEC) {
+    load8(a.bias + c0, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (c0 + e < a.cout) v[e] = a.bias[c0 + e];
+  }
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void residual8(const MmArgs& a, long long row, int c0, float (&v)[8]) {
+  const T* res = reinterpret_cast<const T*>(a.res) + row * a.res_ld + c0;
+  if constexpr (VEC) {
+    load8(res, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = c0 + e < a.cout ? ElemTraits<T>::load(res + e) : 0.f;
+  }
+}
+// Activation and store of 8 consecutive channels of a row that exists.  VEC: cout and the strides allow
+// 16-byte accesses.  (Two kernels instead of a branch: a launch that does little is bound by
+// fetching its instructions.)
 template <typename T, bool VEC>
 __device__ __forceinline__ void finish8(const MmArgs& a, const Limits& lim, long long row, int c0, float (&v)[8]) {
   T* y = reinterpret_cast<T*>(a.y) + row * a.y_ld + c0;
-  const T* res = reinterpret_cast<const T*>(a.res) + row * a.res_ld + c0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = clip(v[e], lim);
   if constexpr (VEC) {
-    if (a.bias != nullptr) {
-      float b[8];
-      load8(a.bias + c0, b);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] += b[e];
-    }
-    if (a.res != nullptr) {
-      float r[8];
-      load8(res, r);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] += r[e];
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = clip(v[e], lim);
     store8(y, v);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (c0 + e < a.cout) {
-        float t = v[e];
-        if (a.bias != nullptr) t += a.bias[c0 + e];
-        if (a.res != nullptr) t += ElemTraits<T>::load(res + e);
-        store1(y + e, clip(t, lim));
-      }
+      if (c0 + e < a.cout) store1(y + e, v[e]);
   }
 }
 
@@ -410,23 +416,43 @@ matmul_fp8_tile_kernel(const MmArgs a, int tiles_n) {
 #pragma unroll
         for (int z = 0; z < WK - 1; ++z) acc[j][i] += part[z * kGroup + (j * TI + i) * 64];
   }
+  // bias once per 8 channels, the residuals of a column before its first store (the compiler would keep each
+  // load behind the stores in front of it)
   const Limits lim = limits_of<T>(a.act);
 #pragma unroll
   for (int i = 0; i < TI; i += 2) {
     const int c0 = (wn * TI + i) * 16 + 8 * g;
     if (c0 >= chans_left) break;
+    float add[TJ][8];
+    if constexpr (!PART) {
+      float bias[8];
+      bias8<T, VEC>(a, n0 + c0, bias);
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) {
+        const int row = (wm * TJ + j) * 16 + r;
+        float res[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (a.res != nullptr && row < rows_left) residual8<T, VEC>(a, m0 + row, n0 + c0, res);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) add[j][e] = bias[e] + res[e];
+      }
+    }
 #pragma unroll
     for (int j = 0; j < TJ; ++j) {
       const int row = (wm * TJ + j) * 16 + r;
+      if (row >= rows_left) continue;
       float v[8];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         v[e] = acc[j][i][e];
         v[4 + e] = acc[j][i + 1][e];
       }
-      if (row >= rows_left) continue;
-      if constexpr (PART) store8(a.part + ((long long)blockIdx.y * a.rows + m0 + row) * a.part_ld + n0 + c0, v);
-      else finish8<T, VEC>(a, lim, m0 + row, n0 + c0, v);
+      if constexpr (PART) {
+        store8(a.part + ((long long)blockIdx.y * a.rows + m0 + row) * a.part_ld + n0 + c0, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += add[j][e];
+        finish8<T, VEC>(a, lim, m0 + row, n0 + c0, v);
+      }
     }
   }
 }
@@ -444,6 +470,15 @@ __global__ void __launch_bounds__(256) matmul_fp8_join_kernel(const MmArgs a) {
   for (int z = 0; z < a.splits; ++z) {
     float t[8];
     load8(a.part + (z * a.rows + row) * a.part_ld + c0, t);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += t[e];
+  }
+  float t[8];
+  bias8<T, VEC>(a, c0, t);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] += t[e];
+  if (a.res != nullptr) {
+    residual8<T, VEC>(a, row, c0, t);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += t[e];
   }
