@@ -416,6 +416,58 @@ matmul_fp8_tile_kernel(const MmArgs a, int tiles_n) {
 #pragma unroll
         for (int z = 0; z < WK - 1; ++z) acc[j][i] += part[z * kGroup + (j * TI + i) * 64];
   }
+  if constexpr (VEC && !PART && sizeof(T) == 2 && TI == 4) {
+    // 16-bit outputs of 64 channels per wave: lanes r and r + 8 exchange their second 8 channels, so that every
+    // store covers whole 128-byte lines (8 rows) instead of halves of 16
+    const Limits lim = limits_of<T>(a.act);
+    const int ca = wn * 64 + 8 * g, cb = ca + 32;
+    const bool upper = (r & 8) != 0, in_a = ca < chans_left, in_b = cb < chans_left;
+    float ba[8], bb[8];
+    bias8<T, VEC>(a, in_a ? n0 + ca : 0, ba);
+    bias8<T, VEC>(a, in_b ? n0 + cb : 0, bb);
+#pragma unroll
+    for (int j = 0; j < TJ; ++j) {
+      const int row = (wm * TJ + j) * 16 + r;
+      const bool row_ok = row < rows_left;
+      float va[8], vb[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        va[e] = acc[j][e >> 2][e & 3] + ba[e];
+        vb[e] = acc[j][2 + (e >> 2)][e & 3] + bb[e];
+      }
+      if (a.res != nullptr && row_ok) {
+        float t[8];
+        if (in_a) {
+          residual8<T, VEC>(a, m0 + row, n0 + ca, t);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) va[e] += t[e];
+        }
+        if (in_b) {
+          residual8<T, VEC>(a, m0 + row, n0 + cb, t);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) vb[e] += t[e];
+        }
+      }
+      unsigned first[4], second[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const unsigned own = Half16<T>::pack2(clip(va[2 * e], lim), clip(va[2 * e + 1], lim));
+        const unsigned other = (unsigned)__builtin_amdgcn_update_dpp(
+            0, (int)Half16<T>::pack2(clip(vb[2 * e], lim), clip(vb[2 * e + 1], lim)), 0x128, 0xf, 0xf, true);   // row_ror:8
+        first[e] = upper ? other : own;
+        second[e] = upper ? own : other;
+      }
+      const int row1 = row & ~8, row2 = row | 8;
+      char* y = reinterpret_cast<char*>(a.y);
+      if (row1 < rows_left && (upper ? in_b : in_a))
+        *reinterpret_cast<uint4*>(y + 2 * ((m0 + row1) * a.y_ld + n0 + (upper ? cb : ca))) =
+            make_uint4(first[0], first[1], first[2], first[3]);
+      if (row2 < rows_left && (upper ? in_a : in_b))
+        *reinterpret_cast<uint4*>(y + 2 * ((m0 + row2) * a.y_ld + n0 + (upper ? ca : cb))) =
+            make_uint4(second[0], second[1], second[2], second[3]);
+    }
+    return;
+  }
   // bias once per 8 channels, the residuals of a column before its first store (the compiler would keep each
   // load behind the stores in front of it)
   const Limits lim = limits_of<T>(a.act);
