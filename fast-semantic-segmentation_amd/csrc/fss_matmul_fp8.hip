@@ -151,14 +151,12 @@ __device__ __forceinline__ void residual8(const MmArgs& a, long long row, int c0
     for (int e = 0; e < 8; ++e) v[e] = c0 + e < a.cout ? ElemTraits<T>::load(res + e) : 0.f;
   }
 }
-// Activation and store of 8 consecutive channels of a row that exists.  VEC: cout and the strides allow
+// Stores 8 consecutive channels of a row that exists.  VEC: cout and the strides allow
 // 16-byte accesses.  (Two kernels instead of a branch: a launch that does little is bound by
 // fetching its instructions.)
 template <typename T, bool VEC>
-__device__ __forceinline__ void finish8(const MmArgs& a, const Limits& lim, long long row, int c0, float (&v)[8]) {
+__device__ __forceinline__ void finish8(const MmArgs& a, long long row, int c0, const float (&v)[8]) {
   T* y = reinterpret_cast<T*>(a.y) + row * a.y_ld + c0;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = clip(v[e], lim);
   if constexpr (VEC) {
     store8(y, v);
   } else {
@@ -416,95 +414,93 @@ matmul_fp8_tile_kernel(const MmArgs a, int tiles_n) {
 #pragma unroll
         for (int z = 0; z < WK - 1; ++z) acc[j][i] += part[z * kGroup + (j * TI + i) * 64];
   }
-  if constexpr (VEC && !PART && sizeof(T) == 2 && TI == 4) {
-    // 16-bit outputs of 64 channels per wave: lanes r and r + 8 exchange their second 8 channels, so that every
-    // store covers whole 128-byte lines (8 rows) instead of halves of 16
-    const Limits lim = limits_of<T>(a.act);
-    const int ca = wn * 64 + 8 * g, cb = ca + 32;
-    const bool upper = (r & 8) != 0, in_a = ca < chans_left, in_b = cb < chans_left;
-    float ba[8], bb[8];
-    bias8<T, VEC>(a, in_a ? n0 + ca : 0, ba);
-    bias8<T, VEC>(a, in_b ? n0 + cb : 0, bb);
+  const Limits lim = limits_of<T>(a.act);
+  // Two 16-byte pieces a and b of every row, at byte offsets oa and ob, as two stores that cover whole lines of
+  // 8 rows instead of parts of 16: lanes r and r + 8 exchange their pieces b (132612 x 2048, k 2048:
+  // 622 against 675 us).
+  auto put2 = [&](char* base, long long ld, int row, int oa, int ob, const uint4& pa, const uint4& pb, bool in_a, bool in_b) {
+    const bool upper = (r & 8) != 0;
+    auto other = [](unsigned w) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)w, 0x128, 0xf, 0xf, true); };   // row_ror:8
+    const uint4 q = make_uint4(other(pb.x), other(pb.y), other(pb.z), other(pb.w));
+    const int row1 = row & ~8, row2 = row | 8;
+    if (row1 < rows_left && (upper ? in_b : in_a))
+      *reinterpret_cast<uint4*>(base + (m0 + row1) * ld + (upper ? ob : oa)) =
+          make_uint4(upper ? q.x : pa.x, upper ? q.y : pa.y, upper ? q.z : pa.z, upper ? q.w : pa.w);
+    if (row2 < rows_left && (upper ? in_a : in_b))
+      *reinterpret_cast<uint4*>(base + (m0 + row2) * ld + (upper ? oa : ob)) =
+          make_uint4(upper ? pa.x : q.x, upper ? pa.y : q.y, upper ? pa.z : q.z, upper ? pa.w : q.w);
+  };
+  // sums of 8 channels with bias and residual, activated
+  auto final8 = [&](int i, int j, int row, int c0, bool ok, const float (&bias)[8], float (&v)[8]) {
 #pragma unroll
-    for (int j = 0; j < TJ; ++j) {
-      const int row = (wm * TJ + j) * 16 + r;
-      const bool row_ok = row < rows_left;
-      float va[8], vb[8];
+    for (int e = 0; e < 8; ++e) v[e] = acc[j][i + (e >> 2)][e & 3] + bias[e];
+    if (a.res != nullptr && ok) {
+      float t[8];
+      residual8<T, VEC>(a, m0 + row, n0 + c0, t);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        va[e] = acc[j][e >> 2][e & 3] + ba[e];
-        vb[e] = acc[j][2 + (e >> 2)][e & 3] + bb[e];
-      }
-      if (a.res != nullptr && row_ok) {
-        float t[8];
-        if (in_a) {
-          residual8<T, VEC>(a, m0 + row, n0 + ca, t);
+      for (int e = 0; e < 8; ++e) v[e] += t[e];
+    }
 #pragma unroll
-          for (int e = 0; e < 8; ++e) va[e] += t[e];
+    for (int e = 0; e < 8; ++e) v[e] = clip(v[e], lim);
+  };
+  if constexpr (PART) {
+#pragma unroll
+    for (int i = 0; i < TI; i += 2) {
+      const int c0 = (wn * TI + i) * 16 + 8 * g;
+#pragma unroll
+      for (int j = 0; j < TJ; ++j)
+        put2(reinterpret_cast<char*>(a.part + (long long)blockIdx.y * a.rows * a.part_ld), a.part_ld * 4ll, (wm * TJ + j) * 16 + r,
+             (n0 + c0) * 4, (n0 + c0) * 4 + 16, __builtin_bit_cast(uint4, acc[j][i]), __builtin_bit_cast(uint4, acc[j][i + 1]),
+             c0 < chans_left, c0 < chans_left);
+    }
+    return;
+  } else if constexpr (VEC && (sizeof(T) == 4 || TI == 4)) {
+    constexpr int STEP = sizeof(T) == 4 ? 2 : 4;       // a piece pair is 8 floats, or 2 x 8 16-bit channels
+#pragma unroll
+    for (int i = 0; i < TI; i += STEP) {
+      const int ca = (wn * TI + i) * 16 + 8 * g, cb = ca + 32;
+      const bool in_a = ca < chans_left, in_b = STEP == 2 ? in_a : cb < chans_left;
+      float ba[8], bb[8];
+      bias8<T, VEC>(a, in_a ? n0 + ca : 0, ba);
+      if constexpr (STEP == 4) bias8<T, VEC>(a, in_b ? n0 + cb : 0, bb);
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) {
+        const int row = (wm * TJ + j) * 16 + r;
+        const bool ok = row < rows_left;
+        float v[8];
+        final8(i, j, row, ca, ok && in_a, ba, v);
+        uint4 p[2];
+        if constexpr (STEP == 4) {
+          store8(reinterpret_cast<T*>(&p[0]), v);
+          final8(i + 2, j, row, cb, ok && in_b, bb, v);
+          store8(reinterpret_cast<T*>(&p[1]), v);
+        } else {
+          store8(reinterpret_cast<T*>(p), v);
         }
-        if (in_b) {
-          residual8<T, VEC>(a, m0 + row, n0 + cb, t);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) vb[e] += t[e];
-        }
+        constexpr int ES = sizeof(T);
+        put2(reinterpret_cast<char*>(a.y), a.y_ld * ES, row, (n0 + ca) * ES, STEP == 4 ? (n0 + cb) * ES : (n0 + ca) * ES + 16,
+             p[0], p[1], in_a, in_b);
       }
-      unsigned first[4], second[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const unsigned own = Half16<T>::pack2(clip(va[2 * e], lim), clip(va[2 * e + 1], lim));
-        const unsigned other = (unsigned)__builtin_amdgcn_update_dpp(
-            0, (int)Half16<T>::pack2(clip(vb[2 * e], lim), clip(vb[2 * e + 1], lim)), 0x128, 0xf, 0xf, true);   // row_ror:8
-        first[e] = upper ? other : own;
-        second[e] = upper ? own : other;
-      }
-      const int row1 = row & ~8, row2 = row | 8;
-      char* y = reinterpret_cast<char*>(a.y);
-      if (row1 < rows_left && (upper ? in_b : in_a))
-        *reinterpret_cast<uint4*>(y + 2 * ((m0 + row1) * a.y_ld + n0 + (upper ? cb : ca))) =
-            make_uint4(first[0], first[1], first[2], first[3]);
-      if (row2 < rows_left && (upper ? in_a : in_b))
-        *reinterpret_cast<uint4*>(y + 2 * ((m0 + row2) * a.y_ld + n0 + (upper ? ca : cb))) =
-            make_uint4(second[0], second[1], second[2], second[3]);
     }
     return;
   }
   // bias once per 8 channels, the residuals of a column before its first store (the compiler would keep each
   // load behind the stores in front of it)
-  const Limits lim = limits_of<T>(a.act);
 #pragma unroll
   for (int i = 0; i < TI; i += 2) {
     const int c0 = (wn * TI + i) * 16 + 8 * g;
     if (c0 >= chans_left) break;
-    float add[TJ][8];
-    if constexpr (!PART) {
-      float bias[8];
-      bias8<T, VEC>(a, n0 + c0, bias);
+    float bias[8], v[TJ][8];
+    bias8<T, VEC>(a, n0 + c0, bias);
 #pragma unroll
-      for (int j = 0; j < TJ; ++j) {
-        const int row = (wm * TJ + j) * 16 + r;
-        float res[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (a.res != nullptr && row < rows_left) residual8<T, VEC>(a, m0 + row, n0 + c0, res);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) add[j][e] = bias[e] + res[e];
-      }
+    for (int j = 0; j < TJ; ++j) {
+      const int row = (wm * TJ + j) * 16 + r;
+      final8(i, j, row, c0, row < rows_left, bias, v[j]);
     }
 #pragma unroll
     for (int j = 0; j < TJ; ++j) {
       const int row = (wm * TJ + j) * 16 + r;
-      if (row >= rows_left) continue;
-      float v[8];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        v[e] = acc[j][i][e];
-        v[4 + e] = acc[j][i + 1][e];
-      }
-      if constexpr (PART) {
-        store8(a.part + ((long long)blockIdx.y * a.rows + m0 + row) * a.part_ld + n0 + c0, v);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += add[j][e];
-        finish8<T, VEC>(a, lim, m0 + row, n0 + c0, v);
-      }
+      if (row < rows_left) finish8<T, VEC>(a, m0 + row, n0 + c0, v[j]);
     }
   }
 }
@@ -534,7 +530,10 @@ __global__ void __launch_bounds__(256) matmul_fp8_join_kernel(const MmArgs a) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += t[e];
   }
-  finish8<T, VEC>(a, limits_of<T>(a.act), row, c0, v);
+  const Limits lim = limits_of<T>(a.act);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = clip(v[e], lim);
+  finish8<T, VEC>(a, row, c0, v);
 }
 
 // 64 x 64 tiles with k split over the grid
