@@ -234,24 +234,24 @@ matmul_fp8_few_kernel(const MmArgs a, int chan_tiles) {
 }
 
 // ------------------------------------------------------------------------------ many rows
-// BM rows x BN channels per workgroup of WM x WN waves.  Blocks of k (128 bytes of every row) are copied to
-// a ring of NS LDS stages, NS - 1 blocks ahead of the products; 16-byte chunks of a row are exchanged by
-// an XOR with the row, so that a fragment's reads spread over all banks.  Rows and channels past the
-// end and the tail of k are filled with zeros by out-of-range offsets.  The
-// scales travel in the same stages (a scalar load in the loop would make every LDS read wait for memory,
-// as both count on one counter): 64 rows per wave, and the tile's weight scales in the next one.
-template <int BM, int BN, int WM, int WN, int WK, int NS> struct MmTile {
+// BM rows x BN channels per workgroup of WM x WN waves (and WK groups of them, which take turns along k).
+// Blocks of k (128 bytes of every row) are copied to one of two LDS stages while the other is multiplied (more
+// stages changed nothing); 16-byte chunks of a row are exchanged by an XOR with the row, so that a
+// fragment's reads spread over all banks.  Rows and channels past the end and the tail of k are filled
+// with zeros by out-of-range offsets.  The scales travel in the same stages (a scalar load in the loop
+// would make every LDS read wait for memory, as both count on one counter): 64 rows per wave, and the
+// tile's weight scales in the next one.
+template <int BM, int BN, int WM, int WN, int WK> struct MmTile {
   static constexpr int kThreads = 64 * WM * WN * WK, kWaves = WM * WN;
   static constexpr int TJ = BM / WM / 16, TI = BN / WN / 16;
   static constexpr int kXPieces = BM / 8 / kWaves, kWPieces = BN / 8 / kWaves;   // 1 KiB each, per wave
-  static constexpr int kPieces = kXPieces + kWPieces;
   static constexpr int kSPieces = BM / 64 + 1;                                   // 256 bytes each, one per wave
   static constexpr int kXBytes = BM * 128, kWBytes = BN * 128;
   static constexpr int kStage = kXBytes + kWBytes + kSPieces * 256;
-  static constexpr int kLds = NS * WK * kStage;
+  static constexpr int kLds = 2 * WK * kStage;
   static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0 && TI % 2 == 0 && kSPieces <= kWaves &&
                     BM % 64 == 0 && BN % (TI * 16) == 0 && 128 % (TI * 16) == 0, "tile shape");
-  static_assert(kLds <= 160 * 1024 && (NS - 2) * (kPieces + 1) <= 63 && NS >= 2 && NS <= 4, "ring");
+  static_assert(kLds <= 160 * 1024, "LDS");
 };
 
 // 64 lanes x 4 bytes to the 256 bytes of LDS at lds_dst
@@ -265,16 +265,16 @@ __device__ __forceinline__ void blds4(unsigned voff, fss_i32x4 rsrc, unsigned ld
       : "memory", "m0");
 }
 
-template <typename T, bool VEC, bool PART, int BM, int BN, int WM, int WN, int WK, int NS>
+template <typename T, bool VEC, bool PART, int BM, int BN, int WM, int WN, int WK>
 __global__ void __launch_bounds__(64 * WM * WN * WK, 2)
 matmul_fp8_tile_kernel(const MmArgs a, int tiles_n) {
-  typedef MmTile<BM, BN, WM, WN, WK, NS> L;
+  typedef MmTile<BM, BN, WM, WN, WK> L;
   constexpr int TJ = L::TJ, TI = L::TI;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const int lane = threadIdx.x & 63, waves = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wk = waves / L::kWaves, wave = waves % L::kWaves;      // group along k, wave of the group
   const int wm = wave / WN, wn = wave % WN;
-  char* ring = smem + wk * NS * L::kStage;                         // each group has a ring of its own
+  char* ring = smem + wk * 2 * L::kStage;                          // each group has stages of its own
   const unsigned ring_base = (unsigned)(size_t)(__attribute__((address_space(3))) char*)ring;
 
   // the tiles of one XCD are neighbours, taken in columns of 8: what runs at a time shares rows
@@ -344,29 +344,16 @@ matmul_fp8_tile_kernel(const MmArgs a, int tiles_n) {
   const char* psx = ring + L::kXBytes + L::kWBytes + (wm * TJ * 16 + r) * 4;
   const char* pw = ring + L::kXBytes + (wn * TI * 16 + r) * 128;
   const char* psw = ring + L::kXBytes + L::kWBytes + BM * 4 + ((n0 & 127) + wn * TI * 16 >> 7) * 4;
-  const bool more = wave <= BM / 64;           // this wave copies scales, too
 
   // blocks wk, wk + WK, ... of k; all groups make the same number of rounds (a round past the end of
   // k deposits zeros), as they share the barriers
   const int rounds = (kcount + WK - 1) / WK;
-#pragma unroll
-  for (int i = 0; i < NS - 1; ++i)
-    if (i < rounds) stage(kb0 + i * WK + wk, ring_base + i * L::kStage);
-  unsigned cur = 0, ahead = (NS - 1) * L::kStage;
-  for (int round = 0; round < rounds; ++round) {
-    // everything but the stages behind this one (those that exist) has landed
-    const int behind = rounds - 1 - round;
-    if (NS > 3 && behind >= 2) {
-      if (more) wait_vmcnt<(NS > 3 ? 2 : 0) * (L::kPieces + 1)>();
-      else wait_vmcnt<(NS > 3 ? 2 : 0) * L::kPieces>();
-    } else if (NS > 2 && behind >= 1) {
-      if (more) wait_vmcnt<(NS > 2 ? 1 : 0) * (L::kPieces + 1)>();
-      else wait_vmcnt<(NS > 2 ? 1 : 0) * L::kPieces>();
-    } else {
-      wait_vmcnt<0>();
-    }
-    __syncthreads();       // ... for every wave, and nobody reads the stage refilled next any more
-    if (round + NS - 1 < rounds) stage(kb0 + (round + NS - 1) * WK + wk, ring_base + ahead);
+  stage(kb0 + wk, ring_base);
+  unsigned cur = 0;
+  for (int round = 0; round < rounds; ++round, cur = L::kStage - cur) {
+    wait_vmcnt<0>();
+    __syncthreads();       // the stage has landed for every wave, and nobody reads the other one any more
+    if (round + 1 < rounds) stage(kb0 + (round + 1) * WK + wk, ring_base + L::kStage - cur);
     const float sw = *reinterpret_cast<const float*>(psw + cur);
     Block<T> fw[TI];
 #pragma unroll
@@ -389,12 +376,10 @@ matmul_fp8_tile_kernel(const MmArgs a, int tiles_n) {
         for (int e = 0; e < 4; ++e) acc[j][i][e] = fmaf(t[e], s, acc[j][i][e]);
       }
     }
-    cur = cur + L::kStage == NS * L::kStage ? 0 : cur + L::kStage;
-    ahead = ahead + L::kStage == NS * L::kStage ? 0 : ahead + L::kStage;
   }
 
   if constexpr (WK > 1) {
-    // the groups' sums are added in a fixed order; the rings are free after the barrier
+    // the groups' sums are added in a fixed order; the stages are free after the barrier
     static_assert(L::kLds >= (WK - 1) * L::kWaves * TJ * TI * 1024, "sums do not fit");
     fss_f32x4* part = reinterpret_cast<fss_f32x4*>(smem) + (wave * TJ * TI) * 64 + lane;
     constexpr int kGroup = L::kWaves * TJ * TI * 64;
@@ -539,9 +524,9 @@ __global__ void __launch_bounds__(256) matmul_fp8_join_kernel(const MmArgs a) {
 // 64 x 64 tiles with k split over the grid
 template <typename T>
 int launch_split(const MmArgs& a, hipStream_t stream) {
-  typedef MmTile<64, 64, 2, 2, 2, 2> L;
+  typedef MmTile<64, 64, 2, 2, 2> L;
   typedef std::conditional_t<sizeof(T) == 4, float, bf16_t> M;            // which products, nothing else
-  const auto kern = matmul_fp8_tile_kernel<M, true, true, 64, 64, 2, 2, 2, 2>;
+  const auto kern = matmul_fp8_tile_kernel<M, true, true, 64, 64, 2, 2, 2>;
   FSS_CHECK_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, L::kLds));
   const int tiles_n = ceil_div(a.cout, 64);
   const dim3 grid((unsigned)((a.rows + 63) / 64 * tiles_n), a.splits);
@@ -554,16 +539,16 @@ int launch_split(const MmArgs& a, hipStream_t stream) {
   return 0;
 }
 
-template <typename T, bool VEC, int BM, int BN, int WM, int WN, int WK, int NS>
+template <typename T, bool VEC, int BM, int BN, int WM, int WN, int WK>
 int launch_tile(const MmArgs& a, hipStream_t stream) {
-  typedef MmTile<BM, BN, WM, WN, WK, NS> L;
+  typedef MmTile<BM, BN, WM, WN, WK> L;
   const int tiles_n = ceil_div(a.cout, BN);
   const long long tiles = (a.rows + BM - 1) / BM * tiles_n;
   FSS_REQUIRE(tiles < 0x7fffffffLL, "too many tiles");
   if (L::kLds > 64 * 1024)
-    FSS_CHECK_HIP(hipFuncSetAttribute((const void*)matmul_fp8_tile_kernel<T, VEC, false, BM, BN, WM, WN, WK, NS>,
+    FSS_CHECK_HIP(hipFuncSetAttribute((const void*)matmul_fp8_tile_kernel<T, VEC, false, BM, BN, WM, WN, WK>,
                                       hipFuncAttributeMaxDynamicSharedMemorySize, L::kLds));
-  hipLaunchKernelGGL((matmul_fp8_tile_kernel<T, VEC, false, BM, BN, WM, WN, WK, NS>), dim3((unsigned)tiles), dim3(L::kThreads), L::kLds,
+  hipLaunchKernelGGL((matmul_fp8_tile_kernel<T, VEC, false, BM, BN, WM, WN, WK>), dim3((unsigned)tiles), dim3(L::kThreads), L::kLds,
                      stream, a, tiles_n);
   FSS_LAUNCH_CHECK();
   return 0;
@@ -602,17 +587,17 @@ int launch_matmul(const MmArgs& a, hipStream_t stream) {
   if (a.splits > 1) return launch_split<T>(a, stream);
 #define FSS_TILE(...) \
   return a.vec ? launch_tile<T, true, __VA_ARGS__>(a, stream) : launch_tile<T, false, __VA_ARGS__>(a, stream)
-  //   256 x 256 where they fill whole rounds of the 256 compute units and k is long enough to hide a tile's
-  //   ends (8192 x 8192, k 8192: 504 against 578; 33153 x 1024, k 2048, 2.03 rounds: 110 against 94);
+  // 256 x 256 where they fill whole rounds of the 256 compute units and k is long enough to hide a tile's
+  // ends (8192 x 8192, k 8192: 485 against 560; 33153 x 1024, k 2048, 2.03 rounds: 110 against 94);
   const long long big = tiles(256, 256), rounds = (big + 255) / 256;
-  if (big >= 240 && big * 10 >= rounds * 256 * 9 && a.kblocks >= 8) FSS_TILE(256, 256, 2, 4, 1, 2);
-  //   128 x 128 from three per compute unit (33153 x 1024, k 2048: 94 against 129; 8385 x 1024, k 1024,
-  //   528 tiles: 24.0 against 21.7);
-  if (tiles(128, 128) >= 768) FSS_TILE(128, 128, 2, 2, 1, 2);
-  //   64 x 64 with two groups of waves along k where the chain of its blocks is what takes the time (2145 x
-  //   512, k 2048: 10.3 against 11.4; 8385 x 256, k 1024: 11.4 against 9.3), else with one.
-  if (tiles(64, 64) <= 512 && a.kblocks >= 8) FSS_TILE(64, 64, 2, 2, 2, 2);
-  FSS_TILE(64, 64, 2, 2, 1, 2);
+  if (big >= 240 && big * 10 >= rounds * 256 * 9 && a.kblocks >= 8) FSS_TILE(256, 256, 2, 4, 1);
+  // 128 x 128 from three per compute unit (33153 x 1024, k 2048: 94 against 129; 8385 x 1024, k 1024,
+  // 528 tiles: 24.0 against 21.7);
+  if (tiles(128, 128) >= 768) FSS_TILE(128, 128, 2, 2, 1);
+  // 64 x 64 with two groups of waves along k where the chain of its blocks is what takes the time (2145 x
+  // 512, k 2048: 10.0 against 11.6; 8385 x 256, k 1024: 11.4 against 9.3), else with one.
+  if (tiles(64, 64) <= 512 && a.kblocks >= 8) FSS_TILE(64, 64, 2, 2, 2);
+  FSS_TILE(64, 64, 2, 2, 1);
 #undef FSS_TILE
 }
 
@@ -623,7 +608,8 @@ size_t workspace_of(const fss_matmul_fp8_desc& d) {
 
 int check_desc(const fss_matmul_fp8_desc* d) {
   FSS_REQUIRE(d != nullptr, "null descriptor");
-  FSS_REQUIRE(d->rows >= 0 && d->cout > 0, "cout must be positive, rows not negative");
+  FSS_REQUIRE(d->rows >= 0 && d->rows < (1ll << 40), "rows must be in [0, 2^40)");
+  FSS_REQUIRE(d->cout > 0 && d->cout < (1 << 28), "cout must be in [1, 2^28)");
   FSS_REQUIRE(d->k > 0 && d->k % 16 == 0, "k must be a positive multiple of 16");
   FSS_REQUIRE(d->out_dtype == FSS_F32 || d->out_dtype == FSS_BF16 || d->out_dtype == FSS_F16 ||
                   d->out_dtype == FSS_F32_BF16X3, "bad out_dtype");

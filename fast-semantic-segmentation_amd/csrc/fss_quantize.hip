@@ -153,7 +153,8 @@ extern "C" int fss_quantize_fp8(const void* x, long long x_ld, void* q, long lon
                                 void* stream) {
   FSS_REQUIRE(dtype == FSS_F32 || dtype == FSS_BF16 || dtype == FSS_F16 || dtype == FSS_F32_BF16X3, "bad dtype");
   FSS_REQUIRE(block_rows == 1 || block_rows == 128, "block_rows must be 1 or 128");
-  FSS_REQUIRE(rows >= 0 && cols > 0 && cols % 16 == 0, "cols must be a positive multiple of 16, rows not negative");
+  FSS_REQUIRE(rows >= 0 && rows < (1ll << 40), "rows must be in [0, 2^40)");
+  FSS_REQUIRE(cols > 0 && cols % 16 == 0, "cols must be a positive multiple of 16");
   if (rows == 0) return 0;
   FSS_REQUIRE(x && q && scales, "null argument");
   const int chunk = dtype == FSS_F32 ? 4 : 8;

@@ -167,7 +167,8 @@ def test_matmul_refusals():
                 dict(out_dtype=-1), dict(x_ld=128), dict(x_ld=260), dict(w_ld=240), dict(w_ld=264), dict(x_ld=1 << 23),
                 dict(w_ld=1 << 23), dict(x_scale_ld=7), dict(w_scale_ld=0), dict(y_ld=23), dict(res_ld=23),
                 dict(out_dtype=_lib.F32_BF16X3, y_ld=28), dict(out_dtype=_lib.F32_BF16X3, cout=20, w_scale_ld=1),
-                dict(out_dtype=_lib.F32_BF16X3, res_ld=28), dict(rows=1 << 50, x_scale_ld=1 << 50)):
+                dict(out_dtype=_lib.F32_BF16X3, res_ld=28), dict(rows=1 << 50, x_scale_ld=1 << 50),
+                dict(rows=1 << 62, x_scale_ld=1 << 62), dict(cout=1 << 28, w_scale_ld=1 << 28, y_ld=1 << 28, res_ld=1 << 28)):
         d = U.matmul_desc(**dict(dict(rows=8, cout=24, k=256, dt='f32', x_scale_ld=8, w_scale_ld=1, x_ld=256, w_ld=256,
                                       y_ld=24, res_ld=24), **bad))
         _refused('fss_matmul_fp8', ctypes.byref(d), *[1 << 12] * 7, None, 0, None)
