@@ -369,7 +369,7 @@ attention_kernel(const AttnArgs a) {
       const int rq = (qt * NW + wave) * 32 + at, tq = rq / a.group, hq = hk * a.group + rq % a.group;
       const T* qp = reinterpret_cast<const T*>(a.q) + b * a.qs[0] + tq * a.qs[1] + hq * a.qs[2];
       const uint8_t* mq = a.mask + b * a.ms[0] + tq * a.ms[1] + hq * a.ms[2];
-      const float mx = __shfl(m, at), sum = __shfl(l, at), fq = __shfl(f, at);
+      const float mx = __shfl(m, at), fq = __shfl(f, at);
       const float shift = mx == -INFINITY ? 0.f : mx;
       constexpr int PER = (DP + 63) / 64;
       float acc[PER];
@@ -400,7 +400,6 @@ attention_kernel(const AttnArgs a) {
                 (unsigned short)pack2_sat<T>(acc[i] * fq, 0.f);
         }
       }
-      (void)sum;
     }
   }
   if constexpr (SPLIT) {
@@ -408,8 +407,6 @@ attention_kernel(const AttnArgs a) {
       a.part_ml[part * 2] = m;
       a.part_ml[part * 2 + 1] = l;
     }
-  }
-  if constexpr (SPLIT) {
     if (done || !row_ok) return;
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt)
@@ -450,6 +447,11 @@ __device__ __forceinline__ void store_joined(const AttnArgs& a, int row, int ch,
   *reinterpret_cast<uint2*>(a.y + 2 * (b * a.ys[0] + r / a.group * a.ys[1] + head * a.ys[2] + ch)) =
       make_uint2(pack2_sat<T>(v.x * f, v.y * f), pack2_sat<T>(v.z * f, v.w * f));
 }
+// Weight of a piece with maximum m and sum l: none without a key of the query; a NaN among its scores, which
+// may have left no maximum, stays one
+__device__ __forceinline__ float piece_weight(const float2& ml, float top) {
+  return ml.y == 0.f || ml.y != ml.y ? ml.y : __builtin_amdgcn_exp2f(ml.x - top);
+}
 __device__ __forceinline__ void add_piece(float4& v, float w, const float4& o) {
   if (w != 0.f) v = make_float4(fmaf(w, o.x, v.x), fmaf(w, o.y, v.y), fmaf(w, o.z, v.z), fmaf(w, o.w, v.w));
 }
@@ -478,7 +480,7 @@ __global__ void __launch_bounds__(256) attention_join_few_kernel(const AttnArgs 
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
   for (int z = 0; z < kFewSplits; ++z) {
-    const float w = z >= a.splits || ml[z].y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml[z].x - top);
+    const float w = z >= a.splits ? 0.f : piece_weight(ml[z], top);
     if (w != 0.f) l = fmaf(w, ml[z].y, l);
     add_piece(v, w, o[z]);
   }
@@ -504,7 +506,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttnArgs a, i
   if (lane == 0) red[wave] = top;
   __syncthreads();
   top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const float w = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - top);     // 0: no key of the query there
+  const float w = piece_weight(ml, top);
   weight[t] = w;
   float l = w == 0.f ? 0.f : w * ml.y;
 #pragma unroll

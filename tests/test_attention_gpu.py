@@ -137,6 +137,19 @@ def test_attention_carries_seen_nan():
 
 
 @gpu
+@pytest.mark.parametrize('lq,lk', [(1, 1000), (40, 40000), (1, 300)])
+def test_attention_carries_a_piece_of_nan(lq, lk):
+    """Where the key axis is cut into pieces: all keys of one are NaN, and a query that is."""
+    q, k, v = tensors(1, lq, lk, 2, 2, 64, 'bf16', seed=2)
+    n = lk // 3
+    k[0, n:2 * n, 1] = float('nan')
+    y = U.attend(q, k, v, 'bf16')
+    assert torch.isnan(y[:, :, 1]).all() and not torch.isnan(y[:, :, 0]).any()
+    q[0, 0, 0] = float('nan')
+    assert torch.isnan(U.attend(q, k, v, 'bf16')[0, 0]).all()
+
+
+@gpu
 def test_attention_empty():
     q, k, v = tensors(2, 5, 0, 2, 2, 64, 'bf16', seed=1)
     assert (U.attend(q, k, v, 'bf16') == 0).all()
