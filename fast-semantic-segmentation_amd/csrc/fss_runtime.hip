@@ -5,6 +5,8 @@
 namespace fss {
 static thread_local std::string g_last_error;
 void set_error(const std::string& msg) { g_last_error = msg; }
+// captures fss_capture_begin has opened on this thread and fss_capture_end has not closed
+static thread_local int g_open_captures = 0;
 }  // namespace fss
 
 using namespace fss;
@@ -82,6 +84,8 @@ int fss_stream_sync(void* stream) {
 }
 
 int fss_device_sync(void) {
+  // refused here: the runtime's own refusal may cost the caller the capture
+  FSS_REQUIRE(g_open_captures == 0, "a stream is being captured by this thread");
   FSS_CHECK_HIP(hipDeviceSynchronize());
   return 0;
 }
@@ -123,12 +127,14 @@ int fss_event_elapsed_ms(void* start, void* stop, float* ms) {
 int fss_capture_begin(void* stream) {
   FSS_REQUIRE(stream != nullptr, "capture needs a non-null stream");
   FSS_CHECK_HIP(hipStreamBeginCapture((hipStream_t)stream, hipStreamCaptureModeThreadLocal));
+  ++g_open_captures;
   return 0;
 }
 
 int fss_capture_end(void* stream, void** graph_exec) {
   FSS_REQUIRE(graph_exec != nullptr, "null argument");
   hipGraph_t graph = nullptr;
+  if (g_open_captures > 0) --g_open_captures;
   FSS_CHECK_HIP(hipStreamEndCapture((hipStream_t)stream, &graph));
   hipGraphExec_t exec = nullptr;
   hipError_t e = hipGraphInstantiate(&exec, graph, nullptr, nullptr, 0);

@@ -43,7 +43,7 @@ from fss.packing import (f32_to_bf16_bits, f32_to_f16_bits, f32_split_bf16_rows,
 from fss.plan_base import (_CODE, _EPC, _ESZ, _OUT_ARGS, _TORCH_DT, DEFAULT_HALF_ACT_SCOPES,
                            DEFAULT_HALF_SCOPES, LNode, Step, Val)
 from fss.plan_conv import ConvLowering
-from fss.plan_schedule import Schedule
+from fss.plan_schedule import Schedule, retire
 from fss.plan_tune import ConvTuning
 
 
@@ -691,11 +691,9 @@ class CompiledGraph(ConvLowering, ConvTuning, Schedule):
 
     def __del__(self):
         try:
-            lib.fss_device_sync()
-            if self.graph_exec is not None:
-                lib.fss_graph_destroy(self.graph_exec)
-            for e in self.events:
-                lib.fss_event_destroy(e)
+            memory = [self.__dict__.get(n) for n in ('_allocs', '_blocks', 'vals', 'temps', 'workspaces', 'keepalive',
+                                                     'input_val')]
+            retire(self.device, self.graph_exec, self.events, memory)
         except Exception:
             pass
 

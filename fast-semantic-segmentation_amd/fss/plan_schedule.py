@@ -18,6 +18,37 @@ from fss.plan_base import (_CODE, _EPC, _ESZ, _OUT_ARGS, _TORCH_DT, DEFAULT_HALF
                            DEFAULT_HALF_SCOPES, LNode, Step, Val)
 
 
+# Plans that have ended and whose device resources still have to go: (device, executable graph, events, what holds the
+# device memory).  An executable graph may be torn down, and memory reused, only when nothing of the plan's
+# last launch is in flight on EITHER of its streams; the plan's stream alone being idle says nothing about the
+# runtime's bookkeeping for the side branch, so the whole device is drained first.  That is a forbidden call while a stream is being
+# captured, and Python may collect a plan at any time, another plan's capture included: then the resources
+# wait here for the end of the capture.
+_retired = []
+_captures = 0               # captures begun by `_capture` and not yet ended
+
+
+def retire(device, graph_exec, events, memory):
+    """Takes over the device resources of a plan that ends, and frees them as soon as that is allowed."""
+    _retired.append((device, graph_exec, events, memory))
+    release_retired()
+
+
+def release_retired():
+    """Frees what ended plans have left, unless a capture is under way (or the device refuses to be drained)."""
+    while _retired and not _captures and not torch.cuda.is_current_stream_capturing():
+        item = _retired.pop()
+        device, graph_exec, events, _ = item
+        with torch.cuda.device(device):
+            if lib.fss_device_sync() != 0:
+                _retired.append(item)
+                return
+            if graph_exec is not None:
+                lib.fss_graph_destroy(graph_exec)
+            for e in events:
+                lib.fss_event_destroy(e)
+
+
 class Schedule(object):
     # ------------------------------------------------------------------ utils
     def _alloc(self, shape, dt, phys_c=None):
@@ -242,21 +273,22 @@ class Schedule(object):
         _lib.call('fss_stream_wait_event', self.sh, self.steps[self.join_after].signal)
 
     def _capture(self):
+        global _captures
         if self.graph_exec is not None:
-            # an executable graph may be torn down only when nothing of its last launch is
-            # still in flight on EITHER stream: the plan's stream alone being idle says
-            # nothing about the runtime's bookkeeping for the side branch, so the whole
-            # device is drained first
-            _lib.call('fss_device_sync')
+            with torch.cuda.device(self.device):
+                _lib.call('fss_device_sync')         # see _retired
             _lib.call('fss_graph_destroy', self.graph_exec)
             self.graph_exec = None
         _lib.call('fss_capture_begin', self.sh)
+        _captures += 1
         ex = ctypes.c_void_p()
         try:
             self.run_eager()
         finally:
+            _captures -= 1
             _lib.call('fss_capture_end', self.sh, ctypes.byref(ex))
         self.graph_exec = ex
+        release_retired()
 
     def _time_launches(self, reps=5):
         for _ in range(2):

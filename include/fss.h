@@ -83,6 +83,8 @@ int fss_memset(void* dst, int value, size_t bytes, void* stream);
 int fss_stream_create(void** stream);
 int fss_stream_destroy(void* stream);
 int fss_stream_sync(void* stream);
+/* Waits for everything on the current device.  Refused (status 2, nothing done) while the calling thread
+ * has a capture open. */
 int fss_device_sync(void);
 
 int fss_event_create(void** event);
@@ -96,7 +98,8 @@ int fss_event_elapsed_ms(void* start, void* stop, float* ms);
 
 /* Stream capture of a whole forward pass into a hipGraph.  Replaces the role
  * of the TF session plan that inference.py:97-98 / libs/evaluator.py:188-199
- * re-run once per image. */
+ * re-run once per image.  A graph is destroyed only when none of its launches is in flight:
+ * fss_device_sync has returned 0 since the last one. */
 int fss_capture_begin(void* stream);
 int fss_capture_end(void* stream, void** graph_exec);
 int fss_graph_launch(void* graph_exec, void* stream);
