@@ -136,6 +136,9 @@ class CompiledGraph(ConvLowering, ConvTuning, Schedule):
             if self.reuse_buffers:
                 self._plan_memory(streams > 1 and use_hip_graph)
             self._lower()
+            # what is still deferred (a frame that a first convolution reads raw) is never wanted again; its
+            # closures hold this plan, which would then end with the cyclic collector only
+            self.lazy = {}
             self._dependencies()                  # every pointer of every launch must resolve
             torch.cuda.synchronize(self.device)   # constants were uploaded on torch's stream
             if autotune:

@@ -18,12 +18,12 @@ from fss.plan_base import (_CODE, _EPC, _ESZ, _OUT_ARGS, _TORCH_DT, DEFAULT_HALF
                            DEFAULT_HALF_SCOPES, LNode, Step, Val)
 
 
-# Plans that have ended and whose device resources still have to go: (device, executable graph, events, what holds the
-# device memory).  An executable graph may be torn down, and memory reused, only when nothing of the plan's
-# last launch is in flight on EITHER of its streams; the plan's stream alone being idle says nothing about the
-# runtime's bookkeeping for the side branch, so the whole device is drained first.  That is a forbidden call while a stream is being
-# captured, and Python may collect a plan at any time, another plan's capture included: then the resources
-# wait here for the end of the capture.
+# What plans that have ended still hold on the device: (device, executable graph, events, owners of the memory).
+# An executable graph may be torn down, and memory reused, only when nothing of the plan's last launch is in
+# flight on EITHER of its streams; the plan's stream alone being idle says nothing about the runtime's
+# bookkeeping for the side branch, so the whole device is drained first.  That is a forbidden call while a
+# stream is being captured, and a plan may end at any time, with the cyclic collector (if it is part of a
+# cycle of its user's) in the middle of another plan's capture: then the resources wait here for its end.
 _retired = []
 _captures = 0               # captures begun by `_capture` and not yet ended
 

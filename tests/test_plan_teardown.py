@@ -191,3 +191,19 @@ def test_plans_collected_during_the_capture_of_others():
             assert np.array_equal(a, b)
         del new, eager, run_eager
         gc.collect()
+
+
+@gpu
+def test_plan_ends_with_its_last_reference():
+    """... and not when the cyclic collector gets round to it."""
+    img = np.random.default_rng(0).integers(0, 256, (1, 256, 512, 3)).astype(np.uint8)
+    gc.collect()
+    gc.disable()
+    try:
+        cg = small_plan()
+        cg.run(img)
+        ended, held = weakref.ref(cg), torch.cuda.memory_allocated()
+        del cg
+        assert ended() is None and torch.cuda.memory_allocated() < held / 2
+    finally:
+        gc.enable()
