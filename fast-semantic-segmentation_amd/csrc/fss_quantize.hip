@@ -44,12 +44,13 @@ __device__ __forceinline__ void scale_of(unsigned amax_bits, float& a, float& sc
 }
 
 // The byte of one element whose quotient 448 x / a lies within 2^-20 of a midpoint: `hi` and `lo` are
-// the two e4m3 neighbours.  Compares 448 |x| with mid * a (both over 512: no overflow): values of T have at
-// most 16 bits (floats 24), so both products, and the side their difference is on, are exact.
+// the two e4m3 neighbours.  Compares 448 |x| with mid * a (both over 512: no overflow).  16-bit types hold at most
+// 11 bits, so that in float 0.875 |x| is exact, and the side that the fused difference is on; floats, and the sums of
+// two bfloat16 values with a gap between them, have up to 24 bits and take both products in double.
 template <typename T> __device__ __forceinline__ unsigned settle(unsigned hi, unsigned lo, float x, float a) {
   const float mid = 0x1p-10f * (fabsf(__builtin_amdgcn_cvt_f32_fp8((int)hi, 0)) + fabsf(__builtin_amdgcn_cvt_f32_fp8((int)lo, 0)));
   float above;
-  if constexpr (__is_same(T, float)) above = (float)(0.875 * fabs((double)x) - (double)mid * (double)a);
+  if constexpr (sizeof(T) == 4) above = (float)(0.875 * fabs((double)x) - (double)mid * (double)a);
   else above = fmaf(-mid, a, 0.875f * fabsf(x));
   return above > 0.f || (above == 0.f && (lo & 1)) ? hi : lo;
 }
