@@ -26,6 +26,7 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kKeys = 64;              // keys per tile
+constexpr float kFar = 256.f;          // see `far` in attention_kernel
 constexpr int kMfma = 0x8, kDsRead = 0x100, kValu = 0x402;     // instruction classes of sched_group_barrier
 
 struct AttnArgs {
@@ -36,7 +37,7 @@ struct AttnArgs {
   const int32_t* lens;
   const uint8_t* mask;
   float* part_o;                       // [splits][all rows][head_dim] sums, not yet divided
-  float* part_ml;                      // [splits][all rows][2]: maximum (log2 units), sum
+  float* part_ml;                      // [splits][all rows][2]: maximum of q . k, sum
   long long qs[3], ks[3], vs[3], ys[3], ms[3];
   int batch, kv_len, kv_heads, group, rows, d, qtiles, splits, negate;
   float c;                             // |scale| * log2(e)
@@ -157,7 +158,12 @@ attention_kernel(const AttnArgs a) {
   f32x16_t o[DP / 32];
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) o[i] = f32x16_t{};
+  // Largest q . k so far and the sum of the p, which are exp2(c q.k - c m): one multiply-add each, the
+  // rounded c m shared by all.  Its error, 2^-24 of itself, is the same factor in the sum and in the output, but far from
+  // zero that factor itself leaves the range of p (f16 q and k of 5000 did).  Where some query of the wave has |c m|
+  // above kFar, m is therefore taken off the scores first, exactly near the maximum.
   float m = -INFINITY, l = 0.f;
+  bool far = false;
 
   // copies a tile to a buffer, 1 KiB pieces dealt to the waves: keys at or behind the length and channels
   // behind head_dim are zeros.  The XOR of a row is the XOR of its piece's first row and of the
@@ -296,17 +302,24 @@ attention_kernel(const AttnArgs a) {
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kt][i]);
-    top = other_half_max(top) * a.c;
+    top = other_half_max(top);
     // the sums are rescaled only where some query's maximum has grown (after a few tiles, hardly ever)
-    if (__any(top > m)) {
-      const float m_new = fmaxf(m, top);
-      const float alpha = __builtin_amdgcn_exp2f(m - (m_new == -INFINITY ? 0.f : m_new));
+    if (__any(top > m) || far) {
+      const float m_new = fmaxf(m, top), base = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = __builtin_amdgcn_exp2f((m - base) * a.c);
       m = m_new;
       l *= alpha;
 #pragma unroll
       for (int i = 0; i < DP / 32; ++i) o[i] *= alpha;
+      far = __any(fabsf(base * a.c) > kFar);
+      if (far) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[kt][i] -= base;
+      }
     }
-    const float m_use = m == -INFINITY ? 0.f : m;
+    const float m_use = far || m == -INFINITY ? 0.f : m * a.c;
     unsigned pf[2][8];
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
@@ -374,7 +387,7 @@ attention_kernel(const AttnArgs a) {
       const T* qp = reinterpret_cast<const T*>(a.q) + b * a.qs[0] + tq * a.qs[1] + hq * a.qs[2];
       const uint8_t* mq = a.mask + b * a.ms[0] + tq * a.ms[1] + hq * a.ms[2];
       const float mx = __shfl(m, at), fq = __shfl(f, at);
-      const float shift = mx == -INFINITY ? 0.f : mx;
+      const float base = mx == -INFINITY ? 0.f : mx;
       constexpr int PER = (DP + 63) / 64;
       float acc[PER];
 #pragma unroll
@@ -388,7 +401,7 @@ attention_kernel(const AttnArgs a) {
 #pragma unroll
         for (int x = 1; x < 64; x <<= 1) dot += __shfl_xor(dot, x);
         const float p = Half16<T>::value(
-            Half16<T>::bits(__builtin_amdgcn_exp2f(fmaf(a.negate ? -dot : dot, a.c, -shift))));
+            Half16<T>::bits(__builtin_amdgcn_exp2f(((a.negate ? -dot : dot) - base) * a.c)));
 #pragma unroll
         for (int i = 0; i < PER; ++i)
           if (lane + 64 * i < a.d) acc[i] = fmaf(p, ElemTraits<T>::load(vp + lane + 64 * i), acc[i]);
@@ -453,14 +466,14 @@ __device__ __forceinline__ void store_joined(const AttnArgs& a, int row, int ch,
 }
 // Weight of a piece with maximum m and sum l: none without a key of the query; a NaN among its scores, which
 // may have left no maximum, stays one
-__device__ __forceinline__ float piece_weight(const float2& ml, float top) {
-  return ml.y == 0.f || ml.y != ml.y ? ml.y : __builtin_amdgcn_exp2f(ml.x - top);
+__device__ __forceinline__ float piece_weight(const float2& ml, float top, float c) {
+  return ml.y == 0.f || ml.y != ml.y ? ml.y : __builtin_amdgcn_exp2f((ml.x - top) * c);
 }
 __device__ __forceinline__ void add_piece(float4& v, float w, const float4& o) {
   if (w != 0.f) v = make_float4(fmaf(w, o.x, v.x), fmaf(w, o.y, v.y), fmaf(w, o.z, v.z), fmaf(w, o.w, v.w));
 }
 
-// Joins few pieces of the key axis, weights 2^(m_z - max m), in index order: one thread per 4 channels.
+// Joins few pieces of the key axis, weights 2^(c (m_z - max m)), in index order: one thread per 4 channels.
 constexpr int kFewSplits = 8;
 
 template <typename T>
@@ -484,7 +497,7 @@ __global__ void __launch_bounds__(256) attention_join_few_kernel(const AttnArgs 
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
   for (int z = 0; z < kFewSplits; ++z) {
-    const float w = z >= a.splits ? 0.f : piece_weight(ml[z], top);
+    const float w = z >= a.splits ? 0.f : piece_weight(ml[z], top, a.c);
     if (w != 0.f) l = fmaf(w, ml[z].y, l);
     add_piece(v, w, o[z]);
   }
@@ -510,7 +523,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttnArgs a, i
   if (lane == 0) red[wave] = top;
   __syncthreads();
   top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const float w = piece_weight(ml, top);
+  const float w = piece_weight(ml, top, a.c);
   weight[t] = w;
   float l = w == 0.f ? 0.f : w * ml.y;
 #pragma unroll
@@ -566,7 +579,7 @@ int check_desc(const fss_attention_desc* d) {
               "q_heads must be a positive multiple of kv_heads");
   FSS_REQUIRE(d->head_dim > 0 && d->head_dim <= 256 && d->head_dim % 8 == 0,
               "head_dim must be a multiple of 8 and at most 256");
-  FSS_REQUIRE(d->scale - d->scale == 0.f, "scale must be finite");
+  FSS_REQUIRE(fabsf(d->scale) < 0x1p127f, "scale must be below 2^127");       // finite in log2 units, too
   FSS_REQUIRE((long long)d->q_len * (d->q_heads / d->kv_heads) < 0x7fff0000LL && d->kv_len < 0x7fff0000, "too long");
   FSS_REQUIRE((long long)d->batch * d->kv_heads *
                       ((long long)d->q_len * (d->q_heads / d->kv_heads) / 32 + 1) < 0x7fff0000LL,

@@ -518,7 +518,8 @@ typedef struct fss_attention_desc {
                                  reads key / value head h / (q_heads / kv_heads) */
   int32_t head_dim;           /* a multiple of 8, at most 256                  */
   int32_t dtype;              /* FSS_BF16 | FSS_F16 (q, k, v and y)             */
-  float scale;                /* of the scores, usually head_dim^-1/2           */
+  float scale;                /* of the scores, usually head_dim^-1/2;
+                                 below 2^127                                  */
   int64_t q_stride[3];        /* batch, token, head, in elements: multiples    */
   int64_t k_stride[3];        /* of 8, not negative, token strides below 2^24  */
   int64_t v_stride[3];
