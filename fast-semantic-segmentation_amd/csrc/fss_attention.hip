@@ -82,6 +82,10 @@ __device__ __forceinline__ float other_half_max(float v) {
   return fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
 }
 
+// p is carried at 2^kUp of its size, which the quotient drops again: half precision then holds p down to 2^-39 of a
+// query's largest (2^-24 as it is), so that many weak keys are not lost one by one
+template <typename T> constexpr float kUp = __is_same(T, f16_t) ? 15.f : 0.f;
+
 typedef __attribute__((address_space(3))) const char* lds_ptr;
 typedef __attribute__((address_space(3))) i16x4_t* lds_tr_ptr;
 __device__ __forceinline__ uint4 lds16(lds_ptr p) {
@@ -319,7 +323,7 @@ attention_kernel(const AttnArgs a) {
           for (int i = 0; i < 16; ++i) s[kt][i] -= base;
       }
     }
-    const float m_use = far || m == -INFINITY ? 0.f : m * a.c;
+    const float m_use = (far || m == -INFINITY ? 0.f : m * a.c) - kUp<T>;
     unsigned pf[2][8];
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
@@ -401,7 +405,7 @@ attention_kernel(const AttnArgs a) {
 #pragma unroll
         for (int x = 1; x < 64; x <<= 1) dot += __shfl_xor(dot, x);
         const float p = Half16<T>::value(
-            Half16<T>::bits(__builtin_amdgcn_exp2f(((a.negate ? -dot : dot) - base) * a.c)));
+            Half16<T>::bits(__builtin_amdgcn_exp2f(fmaf((a.negate ? -dot : dot) - base, a.c, kUp<T>))));
 #pragma unroll
         for (int i = 0; i < PER; ++i)
           if (lane + 64 * i < a.d) acc[i] = fmaf(p, ElemTraits<T>::load(vp + lane + 64 * i), acc[i]);

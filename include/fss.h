@@ -534,10 +534,11 @@ int fss_cross_attention_workspace_bytes(const fss_attention_desc* desc, size_t* 
 /* y[b,i,h] = sum_j p[j] v[b,j,h'] / sum_j p[j],  p[j] = exp(scale * q[b,i,h] . k[b,j,h'] - max)
  * over the keys j < kv_lens[b] (NULL: kv_len; values are clamped to 0 .. kv_len) whose
  * mask[b,i,h,j] is not 0 (uint8, consecutive along j; NULL: all).  A query without any such key
- * gets zeros.  Keys and values at or behind kv_lens[b] are not read; a masked key has no effect
- * whatever its key and value hold, infinities and NaN included.  Scores, maximum, sums and the
- * output are accumulated in float; p is rounded to `dtype` (for the product with v and for the sum
- * alike), y once at the end (FSS_F16 saturates).  q, k, v, y and workspace: 16-byte aligned.
+ * gets zeros, one whose scores are all minus infinity, too.  Keys and values at or behind kv_lens[b]
+ * are not read; a masked key has no effect whatever its key and value hold, infinities and NaN
+ * included.  Scores, maximum, sums and the output are accumulated in float; p is rounded to `dtype`
+ * (for the product with v and for the sum alike; FSS_F16 below 2^-29 of the query's largest p: by up
+ * to 2^-40 of that), y once at the end (FSS_F16 saturates).  q, k, v, y and workspace: 16-byte aligned.
  * kv_lens is read on the device, so a captured call follows its later contents. */
 int fss_cross_attention(const fss_attention_desc* desc, const void* q, const void* k, const void* v,
                         const int32_t* kv_lens, const uint8_t* mask, void* y, void* workspace,

@@ -71,3 +71,35 @@ def test_attention_offset_scores(lq, lk, dt, offset):
     tol = size * (U.HALF[dt] + 2 * p + 4 * u * (lk + 8)) + want.abs() * U.HALF[dt] + 2.0 ** -25
     bad = (y[0] - want[0]).abs() > tol[0]
     assert not bad.any(), (int(bad.sum()), float((y[0] - want[0]).abs().max()))
+
+
+@pytest.mark.parametrize('lq', [3, 150, 66000])
+@pytest.mark.parametrize('dt', ['f16', 'bf16'])
+@pytest.mark.parametrize('masked', [False, True])
+def test_attention_many_weak_keys(lq, dt, masked):
+    """One strong key, of value 0, above 33151 weak ones whose p are below half precision's subnormal numbers: they alone
+    are the result."""
+    if masked and lq > 1000:
+        lq = 16500
+    lk, d, strong = 33152, 8, 5
+    q, k, v = plane(lq, lk, 1 if not masked else 4, d, dt, seed=0)
+    heads = k.shape[2]
+    q[..., 0] = 1.0
+    for t in (-10.0, -14.0, -17.5, -20.0, -23.0):
+        k[..., 0] = t
+        v[:] = 1000.0
+        k[:, strong, :, 0], v[:, strong] = 0.0, 0.0
+        mask = torch.ones(1, 1, 1, lk, dtype=torch.bool, device='cuda').expand(1, heads, lq, lk) if masked else None
+        y = U.attend(q, k, v, dt, scale=1.0, mask=mask).double()
+        weak = (lk - 1) * np.exp(t)
+        want = 1000 * weak / (1 + weak)
+        # p: an exponent of up to 34 with two roundings, its base (2^-16, see above), an exponential of two steps, its
+        # rounding to dt; the sum of the p takes two halves of the keys pair by pair, half a step each at
+        # most; the output 16 keys at a time, a step each; its rounding
+        u = 2.0 ** -24
+        tol = want * (U.HALF[dt] + 2 * (34 * 2 * u + 2.0 ** -16 + 4 * u) + lk / 4 * u + lk / 16 * 2 * u + U.HALF[dt])
+        if dt == 'f16':
+            # Half precision has steps of 2^-24 below 2^-14, of 2^-39 of the largest p below 2^-29 of it as p is
+            # carried: half a step for each weak key, at -23 (2^-33.2) 3.0e-5 in all for a result of 3.4e-3
+            tol += 1000 * (lk - 1) * 2.0 ** -40
+        assert float((y - want).abs().max()) <= tol, (t, float((y - want).abs().max()), tol)
