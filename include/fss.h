@@ -536,7 +536,8 @@ int fss_cross_attention_workspace_bytes(const fss_attention_desc* desc, size_t* 
  * mask[b,i,h,j] is not 0 (uint8, consecutive along j; NULL: all).  A query without any such key
  * gets zeros, one whose scores are all minus infinity, too.  Keys and values at or behind kv_lens[b]
  * are not read; a masked key has no effect whatever its key and value hold, infinities and NaN
- * included.  Scores, maximum, sums and the output are accumulated in float; p is rounded to `dtype`
+ * included (where a value that is not finite is hidden from a query, that query is formed a second
+ * time, some hundred times as slowly; one whose result is NaN as a whole is not).  Scores, maximum, sums and the output are accumulated in float; p is rounded to `dtype`
  * (for the product with v and for the sum alike; FSS_F16 below 2^-29 of the query's largest p: by up
  * to 2^-40 of that), y once at the end (FSS_F16 saturates).  q, k, v, y and workspace: 16-byte aligned.
  * kv_lens is read on the device, so a captured call follows its later contents. */
