@@ -6,6 +6,8 @@
 // byte) and the scales (4 bytes per 128 or 16384 elements) are written once; a block's values stay in
 // registers between its maximum and its conversion.  132612 x 2048 bfloat16: 142 us, 5.8 TB/s; 2048 x 4096
 // floats in 128 x 128 blocks: 8.1 us, 5.2 TB/s; 1 x 512: 3.2 us, a launch.
+#include <algorithm>
+
 #include "fss_common.h"
 
 namespace fss {
@@ -14,6 +16,7 @@ namespace {
 constexpr float kE4m3Max = 448.f;
 constexpr unsigned kTinyBits = 0x0d800000u;      // 2^-100: blocks below it (zeros) share its scale
 constexpr unsigned kInfBits = 0x7f800000u;
+constexpr long long kMaxGrid256 = (1ll << 24) - 1;       // workgroups of 256
 
 // 16 consecutive elements as floats
 template <typename T>
@@ -167,23 +170,32 @@ extern "C" int fss_quantize_fp8(const void* x, long long x_ld, void* q, long lon
   const long long row_blocks = (rows + block_rows - 1) / block_rows;
   FSS_REQUIRE(scale_ld >= row_blocks, "scale_ld is less than the number of row blocks");
   const int col_blocks = ceil_div(cols, 128);
-  const long long groups = (block_rows == 1 ? (rows + 31) / 32 : row_blocks) * col_blocks;
-  FSS_REQUIRE(groups < 0x7fffffffLL, "too many blocks");
+  // A launch holds fewer than 2^32 threads (more are cut off without an error): rows in parts
+  const int unit = block_rows == 1 ? 32 : 128;
+  FSS_REQUIRE(col_blocks <= kMaxGrid256, "too many columns");
+  const long long part = kMaxGrid256 / col_blocks * unit;
   hipStream_t s = (hipStream_t)stream;
-#define FSS_QUANT(T)                                                                                            \
-  do {                                                                                                          \
-    if (block_rows == 1)                                                                                        \
-      hipLaunchKernelGGL(quantize_rows_kernel<T>, dim3((unsigned)groups), dim3(256), 0, s, (const T*)x, x_ld,   \
-                         (uint8_t*)q, q_ld, scales, scale_ld, rows, cols, col_blocks);                          \
-    else                                                                                                        \
-      hipLaunchKernelGGL(quantize_tiles_kernel<T>, dim3((unsigned)groups), dim3(256), 0, s, (const T*)x, x_ld,  \
-                         (uint8_t*)q, q_ld, scales, scale_ld, rows, cols, col_blocks);                          \
+  for (long long r0 = 0; r0 < rows; r0 += part) {
+    const long long n = std::min(part, rows - r0);
+    const dim3 grid((unsigned)((n + unit - 1) / unit * col_blocks));
+#define FSS_QUANT(T)                                                                                                 \
+  do {                                                                                                               \
+    const T* xp = (const T*)x + r0 * x_ld;                                                                           \
+    uint8_t* qp = (uint8_t*)q + r0 * q_ld;                                                                           \
+    float* sp = scales + r0 / block_rows;                                                                            \
+    if (block_rows == 1)                                                                                             \
+      hipLaunchKernelGGL(quantize_rows_kernel<T>, grid, dim3(256), 0, s, xp, x_ld, qp, q_ld, sp, scale_ld, n, cols,  \
+                         col_blocks);                                                                                \
+    else                                                                                                             \
+      hipLaunchKernelGGL(quantize_tiles_kernel<T>, grid, dim3(256), 0, s, xp, x_ld, qp, q_ld, sp, scale_ld, n, cols, \
+                         col_blocks);                                                                                \
   } while (0)
-  if (dtype == FSS_F32) FSS_QUANT(float);
-  else if (dtype == FSS_BF16) FSS_QUANT(bf16_t);
-  else if (dtype == FSS_F16) FSS_QUANT(f16_t);
-  else FSS_QUANT(f32s_t);
+    if (dtype == FSS_F32) FSS_QUANT(float);
+    else if (dtype == FSS_BF16) FSS_QUANT(bf16_t);
+    else if (dtype == FSS_F16) FSS_QUANT(f16_t);
+    else FSS_QUANT(f32s_t);
 #undef FSS_QUANT
-  FSS_LAUNCH_CHECK();
+    FSS_LAUNCH_CHECK();
+  }
   return 0;
 }
