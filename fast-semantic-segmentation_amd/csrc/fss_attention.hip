@@ -657,8 +657,10 @@ int check_desc(const fss_attention_desc* d) {
               "head_dim must be a multiple of 8 and at most 256");
   FSS_REQUIRE(fabsf(d->scale) < 0x1p127f, "scale must be below 2^127");       // finite in log2 units, too
   FSS_REQUIRE((long long)d->q_len * (d->q_heads / d->kv_heads) < 0x7fff0000LL && d->kv_len < 0x7fff0000, "too long");
-  FSS_REQUIRE((long long)d->batch * d->kv_heads *
-                      ((long long)d->q_len * (d->q_heads / d->kv_heads) / 32 + 1) < 0x7fff0000LL,
+  // (a launch holds fewer than 2^32 threads, more are cut off without an error; waves of 32 queries in ones, fours, eights)
+  const long long rows = (long long)d->q_len * (d->q_heads / d->kv_heads);
+  const int waves = rows <= 32 ? 1 : d->head_dim > 128 && rows > 128 ? 8 : 4;
+  FSS_REQUIRE((long long)d->batch * d->kv_heads <= ((1ll << 26) - 1) / (std::max(1, ceil_div(rows, 32 * waves)) * waves),
               "too many query tiles");
   return 0;
 }

@@ -548,7 +548,7 @@ int launch_tile(const MmArgs& a, hipStream_t stream) {
   typedef MmTile<BM, BN, WM, WN, WK> L;
   const int tiles_n = ceil_div(a.cout, BN);
   const long long tiles = (a.rows + BM - 1) / BM * tiles_n;
-  FSS_REQUIRE(tiles < 0x7fffffffLL, "too many tiles");
+  FSS_REQUIRE(tiles < (1ll << 32) / L::kThreads, "too many tiles");        // more threads are cut off without an error
   if (L::kLds > 64 * 1024)
     FSS_CHECK_HIP(hipFuncSetAttribute((const void*)matmul_fp8_tile_kernel<T, VEC, false, BM, BN, WM, WN, WK>,
                                       hipFuncAttributeMaxDynamicSharedMemorySize, L::kLds));
@@ -561,8 +561,7 @@ int launch_tile(const MmArgs& a, hipStream_t stream) {
 template <typename T>
 int launch_few(const MmArgs& a, hipStream_t stream) {
   const int chan_tiles = ceil_div(a.cout, 32);
-  const long long groups = (a.rows + 15) / 16 * chan_tiles;
-  FSS_REQUIRE(groups < 0x7fffffffLL, "too many tiles");
+  const long long groups = (a.rows + 15) / 16 * chan_tiles;                // at most 2560, see few_rows
   hipLaunchKernelGGL(matmul_fp8_few_kernel<T>, dim3((unsigned)groups), dim3(kFewWaves * 64), 0, stream, a, chan_tiles);
   FSS_LAUNCH_CHECK();
   return 0;
@@ -572,7 +571,7 @@ int launch_few(const MmArgs& a, hipStream_t stream) {
 // Few rows, while their work is at most 10 blocks of k per compute unit (1 x 512, k 2048: 5.0 against 7.2;
 // 300 x 1024, k 1024: 8.0 against 6.1).
 bool few_rows(long long rows, int cout, int kblocks) {
-  return (rows + 15) / 16 * ceil_div(cout, 32) * kblocks <= 2560;
+  return (double)((rows + 15) / 16) * ceil_div(cout, 32) * kblocks <= 2560;      // (past 2^63 for rows near 2^40)
 }
 // Pieces of k for the grid, where few 64 x 64 tiles meet a long k: to one workgroup per compute unit, of 8
 // blocks each at least (128 x 128, k 16384: 16 pieces 9.4 against 33.0 us whole; 512 x 512, k 8192: 4 pieces 14.3

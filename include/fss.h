@@ -507,13 +507,16 @@ int fss_matmul_fp8_workspace_bytes(const fss_matmul_fp8_desc* desc, size_t* byte
  * FSS_F32 and FSS_F32_BF16X3 the same values go through the half-precision ones, which sum to float
  * accuracy.  x, w, bias and workspace: 16-byte aligned, y and residual aligned to their element
  * (FSS_F32_BF16X3: 32 bytes), x_ld and w_ld multiples of 16 below 2^23.  bias, residual: NULL =
- * none.  Rows and channels of any number; every sum is taken in a fixed order. */
+ * none.  Rows and channels of any number that one launch holds (rows below 2^30 and rows * cout below
+ * 2^35 always do); every sum is taken in a fixed order. */
 int fss_matmul_fp8(const fss_matmul_fp8_desc* desc, const void* x, const float* x_scales,
                    const void* w, const float* w_scales, const float* bias, const void* residual,
                    void* y, void* workspace, size_t workspace_bytes, void* stream);
 
 typedef struct fss_attention_desc {
-  int32_t batch, q_len, kv_len;
+  int32_t batch, q_len, kv_len; /* batch * q_heads * q_len below 2^31, where the
+                                 queries of a key / value head count in whole
+                                 32s, 128s above 32 and 256s above 128         */
   int32_t q_heads, kv_heads;  /* q_heads a multiple of kv_heads: query head h
                                  reads key / value head h / (q_heads / kv_heads) */
   int32_t head_dim;           /* a multiple of 8, at most 256                  */
