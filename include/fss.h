@@ -501,7 +501,8 @@ int fss_matmul_fp8_workspace_bytes(const fss_matmul_fp8_desc* desc, size_t* byte
 /* y = act( sum_b x_scale[b][m] * w_scale[b][n / 128] * (x[m][b] . w[n][b]) + bias[n] [+ residual[m][n]] )
  * over the blocks b of 128 along k: the product of two tensors fss_quantize_fp8 made, x with
  * block_rows 1 and w with block_rows 128, with fss_conv2d_nhwc's epilogue.  The products of a block
- * are summed on the matrix cores, blocks are scaled and summed in float, the result is rounded once,
+ * are summed on the matrix cores, blocks are scaled (by x_scale * w_scale, formed first: infinite
+ * from 2^128 on, inexact below 2^-126) and summed in float, the result is rounded once,
  * to out_dtype (FSS_F16 saturates).  With 16-bit outputs the 8-bit matrix instructions are used,
  * which drop what lies below 2^-13 of the largest of 8 products (2e-5 of the result's size); with
  * FSS_F32 and FSS_F32_BF16X3 the same values go through the half-precision ones, which sum to float
