@@ -12,9 +12,10 @@
 // be taken in any order as long as V is read in the same one, which the transposing LDS read
 // (ds_read_b64_tr_b16: 4 keys x 16 channels -> 4 keys per lane) does at no cost.
 //
-// 2 x 16 heads of 128, 8385 queries, 8385 and 6288 keys: 1.04 ms, 0.96 PFLOP/s (matrix cores 44 %, exponentials
-// and roundings 46 % of the cycles); 8 heads of 64, 2 x 33153 queries, 50 keys: 32 us, 4.2 TB/s; 8 x 32 heads of
-// 128 in 8 groups, one query, 8385 keys: 50 us, 5.4 TB/s; 8 heads of 32, one query, 2145 keys: 8.7 us.
+// 2 x 16 heads of 128, 8385 queries, 8385 and 6288 keys: 1.05 ms, 0.96 PFLOP/s (matrix cores 50 %, exponentials
+// and roundings 48 % of the cycles); of 64, 8385 keys: 0.72 ms, 0.80; 8 heads of 256, 4096 queries and keys: 0.17 ms,
+// 0.80; 8 heads of 64, 2 x 33153 queries, 50 keys: 31 us, 4.3 TB/s; 8 x 32 heads of 128 in 8 groups, one query, 8385 keys:
+// 51 us, 5.3 TB/s; 8 heads of 32, one query, 2145 keys: 8.6 us.
 #include <algorithm>
 
 #include "fss_conv_args.h"

@@ -11,9 +11,9 @@
 // 16-byte stores straight from the accumulators.  The order of the 128 products inside an MFMA is free (both operands are read in the
 // same one), so a lane simply takes 16-byte pieces g and g + 4 of its row's 128 bytes.
 //
-// 16-bit outputs: 8192 x 8192, k 8192: 490 us, 2.24 PFLOP/s (tile copies through L2 and LDS; the matrix
-// cores are busy 44 % of the cycles); 132612 x 2048, k 2048: 622 us, 1.79 PFLOP/s; 33153 x 256, k 512: 15 us,
-// 2.3 TB/s; 1 x 512, k 2048: 5.0 us.  Float outputs: 8192^3 897 us, 1.23 PFLOP/s.
+// 16-bit outputs: 8192 x 8192, k 8192: 480 us, 2.3 PFLOP/s; 132612 x 2048, k 2048: 588 - 630 us, 1.8 PFLOP/s (all waves drain
+// and meet at every block of k: matrix cores busy 45 % of the cycles, waves at waits and barriers 31 %); 33153 x 256, k
+// 512: 15 us, 2.3 TB/s; 1 x 512, k 2048: 5.0 us.  Float outputs: 8192^3 897 us, 1.23 PFLOP/s.
 #include <algorithm>
 #include <type_traits>
 

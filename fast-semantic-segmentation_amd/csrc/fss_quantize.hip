@@ -4,8 +4,9 @@
 //
 // for blocks of 1 row (activations) or 128 rows (weights).  HBM-bound: x is read once, q (one
 // byte) and the scales (4 bytes per 128 or 16384 elements) are written once; a block's values stay in
-// registers between its maximum and its conversion.  132612 x 2048 bfloat16: 142 us, 5.8 TB/s; 2048 x 4096
-// floats in 128 x 128 blocks: 8.1 us, 5.2 TB/s; 1 x 512: 3.2 us, a launch.
+// registers between its maximum and its conversion.  132612 x 2048 bfloat16: 142 to 157 us, 5.2 to 5.8
+// TB/s, split-bfloat16 232 us, 5.9 TB/s; 2048 x 4096 floats in 128 x 128 blocks: 8.1 us, 5.2 TB/s; 1 x 512: 3.2
+// us, a launch.
 #include <algorithm>
 
 #include "fss_common.h"
