@@ -25,7 +25,7 @@ from fss.plan_base import (_CODE, _EPC, _ESZ, _OUT_ARGS, _TORCH_DT, DEFAULT_HALF
 # stream is being captured, and a plan may end at any time, with the cyclic collector (if it is part of a
 # cycle of its user's) in the middle of another plan's capture: then the resources wait here for its end.
 _retired = []
-_captures = 0               # captures begun by `_capture` and not yet ended
+_captures = []              # streams whose capture `_capture` has begun and not yet ended
 
 
 def retire(device, graph_exec, events, memory):
@@ -273,19 +273,18 @@ class Schedule(object):
         _lib.call('fss_stream_wait_event', self.sh, self.steps[self.join_after].signal)
 
     def _capture(self):
-        global _captures
         if self.graph_exec is not None:
             with torch.cuda.device(self.device):
                 _lib.call('fss_device_sync')         # see _retired
             _lib.call('fss_graph_destroy', self.graph_exec)
             self.graph_exec = None
         _lib.call('fss_capture_begin', self.sh)
-        _captures += 1
+        _captures.append(self.sh)
         ex = ctypes.c_void_p()
         try:
             self.run_eager()
         finally:
-            _captures -= 1
+            _captures.remove(self.sh)
             _lib.call('fss_capture_end', self.sh, ctypes.byref(ex))
         self.graph_exec = ex
         release_retired()
